@@ -114,6 +114,47 @@ class AgeOutDesc(ctypes.Structure):
     ]
 
 
+PLAN_MAX_ROWS = 16384
+MAX_AXES = 4
+
+
+class PlanDesc(ctypes.Structure):
+    _fields_ = [(n, _c_i64) for n in ("R", "total", "page_size", "table_width", "table_stride", "free_cap")] + [
+        (n, _vp) for n in ("new_lens", "kv_lens", "block_table", "free_pages", "n_free", "cu_q", "kv_out", "positions",
+                           "slots", "n_free_out", "status")
+    ]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [
+        *((n, _c_i64) for n in ("dtype", "T", "Hq", "Hkv", "D", "rot", "axes")),
+        *((f"section{a}", _c_i64) for a in range(MAX_AXES)),
+        *((n, _c_i64) for n in ("interleaved", "inverse", "round_tables", "positions_64", "pos_stride")),
+        ("positions", _vp), ("inv_freq", _vp),
+        ("q", _vp), ("q_st", _c_i64), ("q_sh", _c_i64),
+        ("q_out", _vp), ("qo_st", _c_i64), ("qo_sh", _c_i64),
+        ("k", _vp), ("k_st", _c_i64), ("k_sh", _c_i64),
+        ("v", _vp), ("v_st", _c_i64), ("v_sh", _c_i64),
+        ("slots", _vp), ("page_size", _c_i64), ("n_pages", _c_i64),
+        ("k_pool", _vp), ("kp_sp", _c_i64), ("kp_sh", _c_i64), ("kp_st", _c_i64),
+        ("v_pool", _vp), ("vp_sp", _c_i64), ("vp_sh", _c_i64), ("vp_st", _c_i64),
+    ]
+
+
+class ChunkDesc(ctypes.Structure):
+    _fields_ = [
+        *((n, _c_i64) for n in ("dtype", "R", "T", "Hq", "Hkv", "D", "page_size", "n_pages", "table_width",
+                                "table_stride", "causal", "window")),
+        ("sm_scale", ctypes.c_double),
+        ("q", _vp), ("q_st", _c_i64), ("q_sh", _c_i64),
+        ("out", _vp), ("o_st", _c_i64), ("o_sh", _c_i64),
+        ("lse", _vp),
+        ("k_pool", _vp), ("kp_sp", _c_i64), ("kp_sh", _c_i64), ("kp_st", _c_i64),
+        ("v_pool", _vp), ("vp_sp", _c_i64), ("vp_sh", _c_i64), ("vp_st", _c_i64),
+        ("block_table", _vp), ("cu_q", _vp), ("kv_lens", _vp),
+    ]
+
+
 # (name, restype, argtypes) for every symbol of include/fade_b200.h
 _SIGNATURES = {
     "fade_status_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -170,6 +211,14 @@ _SIGNATURES = {
     "fade_decode_attn_noalloc_check": (ctypes.c_int, [_vp]),
     "fade_set_middle_kernel": (ctypes.c_int, [ctypes.c_int]),
     "fade_get_middle_kernel": (ctypes.c_int, []),
+    "fade_plan_step": (ctypes.c_int, [ctypes.POINTER(PlanDesc), _vp]),
+    "fade_release_rows": (
+        ctypes.c_int,
+        [_vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _vp],
+    ),
+    "fade_rope_axes": (ctypes.c_int, [ctypes.POINTER(RopeDesc), _vp]),
+    "fade_chunk_attn_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(ChunkDesc)]),
+    "fade_chunk_attn": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _vp, ctypes.c_size_t, _vp]),
 }
 
 _lib = None

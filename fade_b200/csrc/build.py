@@ -17,7 +17,7 @@ from pathlib import Path
 CSRC = Path(__file__).resolve().parent
 PKG = CSRC.parent
 LIB_NAME = "libfade_sm100.so"
-SOURCES = ("abi.cu", "quant.cu", "rotate.cu", "rope.cu", "decode.cu")
+SOURCES = ("abi.cu", "quant.cu", "rotate.cu", "rope.cu", "paged.cu", "chunk_attn.cu", "decode.cu")
 
 NVCC_FLAGS = [
     "-O3",

@@ -164,10 +164,15 @@ class Proportional(RopeScheme):
 @dataclass
 class MRope(RopeScheme):
     """Multi-resolution RoPE; for text the three position axes coincide, so
-    the tables are vanilla RoPE over ``rotary_dim`` (zero angles beyond)."""
+    the tables are vanilla RoPE over ``rotary_dim`` (zero angles beyond).
+    Positions of several axes ([A, S], time, height, width) give each
+    frequency the angle of its axis: ``mrope_section`` frequencies per axis in
+    order, or ``interleaved`` (``fade_b200.paged.rope_axes`` applies the same
+    angles without tables)."""
 
     partial_rotary_factor: float = 1.0
     mrope_section: list | None = None
+    interleaved: bool = False
 
     @property
     def rotary_dim(self) -> int:
@@ -177,7 +182,16 @@ class MRope(RopeScheme):
         return _base_inv_freq(self.rotary_dim, self.rotary_dim, self.theta, device)
 
     def compute_cos_sin(self, positions, device, model_dtype=torch.float16):
-        f = positions.to(device).float()[:, None] * self.inv_freq(device)[None, :]
+        if positions.dim() == 2:
+            from fade_b200.paged import section_axes
+
+            if self.mrope_section is None or len(self.mrope_section) != positions.shape[0]:
+                raise ValueError(f"positions of {positions.shape[0]} axes need an mrope_section of as many entries, "
+                                 f"got {self.mrope_section}")
+            axes = torch.tensor(section_axes(self.mrope_section, self.interleaved), device=device)
+            f = positions.to(device).float()[axes].t() * self.inv_freq(device)[None, :]
+        else:
+            f = positions.to(device).float()[:, None] * self.inv_freq(device)[None, :]
         a = torch.cat((f, f), dim=-1)
         if self.rotary_dim < self.head_dim:
             a = torch.cat([a, torch.zeros(a.shape[0], self.head_dim - self.rotary_dim, device=device)], dim=-1)
@@ -252,7 +266,8 @@ def extract_rope_scheme(cfg, head_dim: int | None = None) -> RopeScheme:
         section = getattr(cfg, "mrope_section", None)
     if section is not None:
         prf = float(rp.get("partial_rotary_factor", 1.0)) if isinstance(rp, dict) else 1.0
-        return MRope(theta=theta, head_dim=hd, partial_rotary_factor=prf, mrope_section=list(section))
+        inter = bool(rp.get("mrope_interleaved", False)) if isinstance(rp, dict) else False
+        return MRope(theta=theta, head_dim=hd, partial_rotary_factor=prf, mrope_section=list(section), interleaved=inter)
     rs = getattr(cfg, "rope_scaling", None)
     if not isinstance(rs, dict):
         return Vanilla(theta=theta, head_dim=hd)

@@ -336,6 +336,131 @@ int fade_get_middle_kernel(void);
  * stream).  Returns FADE_OK or FADE_ERR_TIMEOUT. */
 int fade_workspace_check(void* workspace, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Serving step over a paged FP16/BF16 cache (no counterpart in the           */
+/* reference, which keeps one dense cache per batch): page planning, rotary   */
+/* positions with several axes fused with the append to the pages, and        */
+/* attention of the step's new tokens over the pages.                          */
+/* ------------------------------------------------------------------------ */
+
+/* Codes of the device status word of fade_plan_step / fade_release_rows. */
+typedef enum fade_plan_status {
+    FADE_PLAN_OK = 0,
+    FADE_PLAN_NO_PAGES = 1,   /* the free list holds too few pages            */
+    FADE_PLAN_ROW_FULL = 2,   /* a request needs more pages than a table row  */
+    FADE_PLAN_TOKENS = 3,     /* more new tokens than `total`                 */
+    FADE_PLAN_LENGTHS = 4     /* a negative length or count                   */
+} fade_plan_status;
+
+/* One step of page planning for R requests (at most FADE_PLAN_MAX_ROWS).
+ * Inputs (device): new_lens, kv_lens int32 [R] (new tokens of this step, tokens
+ * cached before it); free_pages int32 [free_cap], a stack whose first n_free[0]
+ * entries are free; block_table int32 [R, table_width] with rows table_stride
+ * apart, its first ceil(kv_lens[r]/page_size) entries per row valid.
+ * With need_r = ceil((kv+new)/page_size) - ceil(kv/page_size), requests in
+ * order, the k-th page handed out is free_pages[n_free-1-k]; it is written into
+ * the table.  Outputs (device, none may alias an input):
+ *   cu_q int32 [R+1], kv_out int32 [R] = kv + new, n_free_out int32 [1],
+ *   positions int32 [total] and slots int64 [total]: token t of request r sits
+ *   at position kv_lens[r] + t - cu_q[r] and in cache slot
+ *   page * page_size + position % page_size; tokens past cu_q[R] get 0 and -1;
+ *   status int32 [1]: a fade_plan_status.  If it is not FADE_PLAN_OK nothing is
+ *   handed out: kv_out = kv_lens, n_free_out = n_free, cu_q 0, every slot -1 and
+ *   the table untouched.
+ * page_size: a power of two.  No host synchronisation. */
+#define FADE_PLAN_MAX_ROWS 16384
+typedef struct fade_plan_desc {
+    int64_t R, total, page_size, table_width, table_stride, free_cap;
+    const int32_t* new_lens;
+    const int32_t* kv_lens;
+    int32_t* block_table;
+    const int32_t* free_pages;
+    const int32_t* n_free;
+    int32_t* cu_q;
+    int32_t* kv_out;
+    int32_t* positions;
+    int64_t* slots;
+    int32_t* n_free_out;
+    int32_t* status;
+} fade_plan_desc;
+int fade_plan_step(const fade_plan_desc* d, void* stream);
+
+/* Gives the pages of finished requests back, in place: for every r with
+ * rows[r] != 0 (u8 [R]), in order, its ceil(kv_lens[r]/page_size) table entries
+ * are pushed onto free_pages (capacity free_cap) and kv_lens[r] becomes 0;
+ * n_free[0] grows.  status as for fade_plan_step; FADE_PLAN_NO_PAGES here means
+ * the stack would overflow.  Nothing changes unless it is FADE_PLAN_OK. */
+int fade_release_rows(const uint8_t* rows, int64_t R, int32_t* kv_lens, const int32_t* block_table,
+                      int64_t table_width, int64_t table_stride, int64_t page_size,
+                      int32_t* free_pages, int64_t free_cap, int32_t* n_free, int32_t* status, void* stream);
+
+/* Rotary positions with several axes.  Frequency j < rot/2 belongs to axis a(j):
+ * sections[0..axes) frequencies per axis one after the other, or interleaved
+ * (a = j mod axes where that is nonzero and j < axes * sections[a], else axis
+ * 0).  angle = fp32(positions[a(j)][t]) * inv_freq[j]; with c, s its cos and sin
+ * (rounded through dtype when round_tables, as the model-side tables of 16-bit
+ * models are),
+ *   y[j] = x[j]*c - x[j+rot/2]*s,  y[j+rot/2] = x[j+rot/2]*c + x[j]*s
+ * in fp32 (products and sums rounded separately), one rounding at the store;
+ * inverse = 1 negates s; channels rot..D-1 are copied.
+ * q [T,Hq,D] -> q_out (may be q itself).  With Hkv > 0: k is rotated likewise
+ * and, with v as it is, written to cache slot slots[t] of k_pool / v_pool
+ * (element (page, head, token) at page*sp + head*sh + token*st); slots outside
+ * [0, n_pages * page_size) are dropped.  All strides in elements, channels
+ * contiguous.  dtype F16, BF16 or F32; positions int32, or int64 with
+ * positions_64 = 1, rows of an axis pos_stride apart. */
+#define FADE_MAX_AXES 4
+typedef struct fade_rope_desc {
+    int64_t dtype, T, Hq, Hkv, D, rot, axes;
+    int64_t sections[FADE_MAX_AXES];
+    int64_t interleaved, inverse, round_tables, positions_64, pos_stride;
+    const void* positions;
+    const float* inv_freq;
+    const void* q;      int64_t q_st, q_sh;
+    void* q_out;        int64_t qo_st, qo_sh;
+    const void* k;      int64_t k_st, k_sh;
+    const void* v;      int64_t v_st, v_sh;
+    const int64_t* slots;
+    int64_t page_size, n_pages;
+    void* k_pool;       int64_t kp_sp, kp_sh, kp_st;
+    void* v_pool;       int64_t vp_sp, vp_sh, vp_st;
+} fade_rope_desc;
+int fade_rope_axes(const fade_rope_desc* d, void* stream);
+
+/* Attention of R requests' new tokens over their paged caches.
+ * q [T,Hq,D] holds the requests' tokens one after the other (cu_q int32 [R+1]);
+ * kv_lens int32 [R] counts a request's cached tokens, the new ones included;
+ * token j of request r lives in page block_table[r][j / page_size] of the pools
+ * (element (page, head, token) at page*sp + head*sh + token*st).  Query i of
+ * request r sits at position p = kv_len - q_len + i and sees the keys
+ *   j < kv_len, causal: j <= p, window > 0: j > p - window.
+ * out[t,hq] = softmax(sm_scale q k^T) v over them with kv head hq / (Hq/Hkv),
+ * lse (nullable, fp32 [T,Hq]) = log sum exp(sm_scale q k); a query that sees no
+ * key gets 0 and -inf.  Rows of q past cu_q[R] are left alone in out and lse.
+ * Cache contents past kv_lens (the rest of the last page, other pages) are never
+ * used, whatever they hold.
+ * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
+ * every pointer and stride of q, k_pool, v_pool and out a multiple of 16 bytes
+ * (else FADE_ERR_ALIGN), sm_scale > 0. */
+typedef struct fade_chunk_desc {
+    int64_t dtype, R, T, Hq, Hkv, D, page_size, n_pages, table_width, table_stride;
+    int64_t causal, window;
+    double sm_scale;
+    const void* q;      int64_t q_st, q_sh;
+    void* out;          int64_t o_st, o_sh;
+    float* lse;
+    const void* k_pool; int64_t kp_sp, kp_sh, kp_st;
+    const void* v_pool; int64_t vp_sp, vp_sh, vp_st;
+    const int32_t* block_table;
+    const int32_t* cu_q;
+    const int32_t* kv_lens;
+} fade_chunk_desc;
+
+/* Bytes of workspace fade_chunk_attn needs for `d` (0: unsupported).  Zero-fill
+ * it once when allocating it; fade_workspace_check reads its error word. */
+size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d);
+int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
