@@ -2,53 +2,806 @@
 //
 // With s_j = sm_scale * q.k_j over the keys a query sees,
 //   out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  lse = m + log sum_j exp(s_j - m)
-// in one pass over the keys, with the running maximum m.
+// in one pass over the keys: scores S = Q K^T and the sum O += P V run on the
+// tensor cores with S, P and O in tensor memory, the running maximum m and the
+// sum of the weights stay in fp32 registers.  P is rounded to the model dtype
+// for its product (as K and V are stored); everything else is fp32 until the
+// one rounding of the result.
+//
+// Rows.  The query heads of a kv head share its keys, so a row is (token, head
+// of the group): row = token * g + head.  A half tile is 128 rows (the M of one
+// MMA): tq = 128 / g tokens; a tile is two half tiles.  Each of two softmax
+// warpgroups owns one *stream*: a score tile (128 rows x 128 keys), a weight
+// tile over it and an output tile in tensor memory, one row per thread.
+//   - more than tq tokens: stream s is half tile s, both walk all key blocks
+//     and share every loaded K and V block;
+//   - up to tq tokens (decodes, drafts, the end of a chunk): both streams hold
+//     the same rows and take alternate key blocks; the two outputs are joined
+//     at the end.
+// While one stream's softmax runs, the tensor cores work on the other's.
+//
+// Work split.  Every (request, kv head, tile) costs its visible keys plus a
+// constant; the sum is cut into equal parts, one per SM, wherever that falls
+// in a tile's keys (to the block of 128).  A CTA walks its contiguous range of
+// tiles; a tile that crosses a cut leaves partial outputs in the workspace,
+// joined by a second kernel.  So ragged batches, the causal triangle and few
+// long rows all fill the GPU alike, from lengths that only the device knows.
+//
+// Warps of a CTA: 0-3 and 4-7 softmax, 8 loads (TMA, one box per page), 9 MMA.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace fade {
 
-// One warp per (token, query head), channels over the lanes, keys one by one.
+constexpr int kBlk = 128;              // keys per block
+constexpr int kHalf = 128;             // rows of a half tile
+constexpr int kCaThreads = 320;
+constexpr int kCaSmemMax = 232448;     // 227 KB
+constexpr int kTileCost = 128;         // fixed cost of a tile, in keys
+constexpr int kMinShare = 256;         // least work of a CTA, in keys: one block per stream
+constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the maximum is moved
+constexpr uint32_t kCaPolls = 1u << 22;
+constexpr int kJoinRows = 8;           // rows per CTA of the joining kernel
+
+struct ChunkParams {
+    const int32_t* block_table;
+    const int32_t* cu_q;
+    const int32_t* kv_lens;
+    void* out;
+    float* lse;
+    int* err;
+    int4* rec;          // [CTA][2][2]: partial segments (continued tile, begun tile)
+    float2* part_ml;    // [CTA][2][256]: (maximum in the log2 domain, sum)
+    float* part_o;      // [CTA][2][256][D]
+    int64_t table_stride, o_st, o_sh;
+    int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window;
+    float scale_log2;
+};
+
+// ---------------------------------------------------------------------------
+// Work split: costs of tiles and their prefix sums
+// ---------------------------------------------------------------------------
+struct Req {
+    int q0, qlen, kv, off;   // first token, tokens, keys, position of the first token
+};
+__device__ __forceinline__ Req load_req(const ChunkParams& p, int b) {
+    Req r;
+    const int c0 = p.cu_q[b], c1 = p.cu_q[b + 1];
+    r.q0 = c0;
+    r.qlen = c0 >= 0 && c1 <= p.T && c1 > c0 ? c1 - c0 : 0;
+    r.kv = min(max(p.kv_lens[b], 0), p.table_width << p.page_log2);
+    r.off = r.kv - r.qlen;
+    return r;
+}
+// sum over i < n of clamp(a + i t, 0, L)
+__device__ __forceinline__ int64_t clamped_sum(int a, int t, int L, int n) {
+    const int n0 = a >= 0 ? 0 : (int)min((uint32_t)n, ((uint32_t)(-a) + t - 1) / t);
+    const int n1 = a >= L ? 0 : (int)min((uint32_t)n, ((uint32_t)L - (uint32_t)a + t - 1) / t);
+    const int64_t m = max(n1 - n0, 0);
+    return a * m + t * (((int64_t)n0 + n1 - 1) * m / 2) + (int64_t)L * (n - max(n1, n0));
+}
+// cost of the first n tiles of a request (for one kv head)
+__device__ __forceinline__ int64_t tiles_cost(const ChunkParams& p, const Req& r, int n) {
+    const int t = 2 * p.tq;
+    int64_t c = (int64_t)kTileCost * n;
+    c += p.causal ? clamped_sum(r.off + t, t, r.kv, n) : (int64_t)r.kv * n;
+    if (p.window > 0) c -= clamped_sum(r.off - p.window + 1, t, r.kv, n);
+    return c;
+}
+__device__ __forceinline__ int tiles_of(const ChunkParams& p, const Req& r) {
+    return (r.qlen + 2 * p.tq - 1) / (2 * p.tq);
+}
+
+// A tile, or the part of its key blocks that a CTA works on.
+struct Seg {
+    Req r;
+    int b, h, i, n;            // request, kv head, tile, its tokens
+    int t0;                    // its first token, within the request
+    int lo_blk, hi_blk;        // key blocks of the tile
+    int k0, k1;                // of this segment
+    __device__ bool whole() const { return k0 == lo_blk && k1 == hi_blk; }
+};
+
+struct Walk {
+    Req r;
+    int b, h, i, nt;
+    int64_t pos, x1, x0;       // cost position of the tile, range of the CTA
+
+    __device__ __forceinline__ bool next(const ChunkParams& p, Seg& s) {
+        while (pos < x1) {
+            const int t = 2 * p.tq;
+            s.r = r;
+            s.b = b, s.h = h, s.i = i;
+            s.t0 = i * t;
+            s.n = min(t, r.qlen - s.t0);
+            const int hi = p.causal ? min(max(r.off + s.t0 + s.n, 0), r.kv) : r.kv;
+            const int lo = p.window > 0 ? min(max(r.off + s.t0 - p.window + 1, 0), hi) : 0;
+            s.lo_blk = lo / kBlk;
+            s.hi_blk = hi > lo ? (hi + kBlk - 1) / kBlk : s.lo_blk;
+            const int cost = kTileCost + hi - lo;
+            auto cut = [&](int64_t x) {
+                const int64_t y = x - pos;
+                if (y <= 0) return s.lo_blk;
+                if (y >= cost) return s.hi_blk;
+                return min(max((lo + max((int)y - kTileCost, 0)) / kBlk, s.lo_blk), s.hi_blk);
+            };
+            s.k0 = cut(x0);
+            s.k1 = cut(x1);
+            const bool owns_start = pos >= x0;
+            pos += cost;
+            if (++i == nt) {
+                i = 0;
+                if (++h == p.Hkv) {
+                    h = 0;
+                    while (pos < x1 && ++b < p.R) {
+                        r = load_req(p, b);
+                        if (r.qlen > 0) break;
+                    }
+                    nt = tiles_of(p, r);
+                }
+            }
+            if (s.k1 > s.k0 || (s.lo_blk == s.hi_blk && owns_start)) return true;
+        }
+        return false;
+    }
+};
+
+// ---------------------------------------------------------------------------
+// Device helpers
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ bool ca_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    for (uint32_t i = 0; i < kCaPolls; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && *abort_flag) return false;
+    }
+    *abort_flag = 1;
+    atomicExch(err, 1);
+    return false;
+}
+__device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+#define CA_R32(v, o)                                                                                              \
+    "=r"(v[o + 0]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), \
+        "=r"(v[o + 7]), "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]),         \
+        "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]),      \
+        "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]),      \
+        "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]),      \
+        "=r"(v[o + 31])
+#define CA_RW32(v, o)                                                                                             \
+    "+r"(v[o + 0]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), \
+        "+r"(v[o + 7]), "+r"(v[o + 8]), "+r"(v[o + 9]), "+r"(v[o + 10]), "+r"(v[o + 11]), "+r"(v[o + 12]),         \
+        "+r"(v[o + 13]), "+r"(v[o + 14]), "+r"(v[o + 15]), "+r"(v[o + 16]), "+r"(v[o + 17]), "+r"(v[o + 18]),      \
+        "+r"(v[o + 19]), "+r"(v[o + 20]), "+r"(v[o + 21]), "+r"(v[o + 22]), "+r"(v[o + 23]), "+r"(v[o + 24]),      \
+        "+r"(v[o + 25]), "+r"(v[o + 26]), "+r"(v[o + 27]), "+r"(v[o + 28]), "+r"(v[o + 29]), "+r"(v[o + 30]),      \
+        "+r"(v[o + 31])
+// 32 columns of this warp's 32 lanes; the values may be read after tc_wait_ld32 on them
+template <int N>
+__device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t (&v)[N], int o) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : CA_R32(v, o)
+        : "r"(taddr)
+        : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tc_wait_ld32(uint32_t (&v)[N], int o) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : CA_RW32(v, o) : : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[N], int o) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(v[o + 0]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]),
+        "r"(v[o + 7]), "r"(v[o + 8]), "r"(v[o + 9]), "r"(v[o + 10]), "r"(v[o + 11]), "r"(v[o + 12]), "r"(v[o + 13]),
+        "r"(v[o + 14]), "r"(v[o + 15]), "r"(v[o + 16]), "r"(v[o + 17]), "r"(v[o + 18]), "r"(v[o + 19]),
+        "r"(v[o + 20]), "r"(v[o + 21]), "r"(v[o + 22]), "r"(v[o + 23]), "r"(v[o + 24]), "r"(v[o + 25]),
+        "r"(v[o + 26]), "r"(v[o + 27]), "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
+        : "memory");
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if (DT == FADE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// Instruction descriptor, kind::f16: f32 accumulator, A and B in the model dtype, M = 128, N columns;
+// b_mn: B is MN-major.
+template <int DT>
+__host__ __device__ constexpr uint32_t ca_idesc(int n, bool b_mn) {
+    return (1u << 4) | ((DT == FADE_BF16 ? 1u : 0u) << 7) | ((DT == FADE_BF16 ? 1u : 0u) << 10) |
+           ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void wg_bar(int id, int threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Shared memory.  Q, K and V tiles are 128 rows of 128 bytes (64 channels) in
+// the 128-byte swizzle, one such sub-tile per 64 channels.
+template <int D>
+struct CaLayout {
+    static constexpr int SUB = 128 * 128;                  // a sub-tile
+    static constexpr int TILE = SUB * (D / 64);            // 128 rows of D channels
+    static constexpr int Q_OFF = 0;
+    static constexpr int RING_OFF = 2 * TILE;
+    static constexpr int NS = D == 128 ? 5 : 11;           // ring stages, one K or V block each
+    static constexpr int ML_OFF = RING_OFF + NS * TILE;    // (m, l) of both streams
+    static constexpr int BAR_OFF = ML_OFF + 2 * 128 * 8;
+    static constexpr int N_BARS = 2 * NS + 10;
+    static constexpr int MISC_OFF = BAR_OFF + 8 * N_BARS;  // tensor-memory slot, abort flag
+    static constexpr int BYTES = MISC_OFF + 16;
+    static_assert(BYTES <= kCaSmemMax, "chunk attention shared memory over the per-CTA limit");
+};
+constexpr int kColS = 0;      // two score tiles of 128 columns; the weights overlay the first 64 of each
+constexpr int kColO = 256;    // two output tiles of D columns
+
 template <int DT, int D>
-__global__ void __launch_bounds__(128) chunk_attn_kernel(const fade_chunk_desc d) {
+__global__ void __launch_bounds__(kCaThreads, 1)
+    chunk_attn_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                      const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ ChunkParams p) {
+    using L = CaLayout<D>;
     using T = typename Elem<DT>::T;
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const int64_t w = blockIdx.x * 4LL + (threadIdx.x >> 5);
-    if (w >= d.T * d.Hq) return;
-    const int64_t t = w / d.Hq, h = w % d.Hq, hk = h / (d.Hq / d.Hkv);
-    int r = -1;
-    for (int i = 0; i < d.R; ++i)
-        if (d.cu_q[i] <= t && t < d.cu_q[i + 1]) r = i;
-    if (r < 0) return;
-    const int64_t kv = min((int64_t)d.kv_lens[r], d.table_width * d.page_size);
-    const int64_t p = kv - d.cu_q[r + 1] + t;
-    const int64_t j1 = d.causal ? min(kv, p + 1) : kv, j0 = d.window > 0 ? max((int64_t)0, p - d.window + 1) : 0;
-    float q[E], acc[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) {
-        q[e] = Elem<DT>::to_f(static_cast<const T*>(d.q)[t * d.q_st + h * d.q_sh + lane * E + e]);
-        acc[e] = 0.f;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t sb = smem_u32(smem);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int cta = blockIdx.x, G = gridDim.x;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 8);
+    const uint32_t bars = sb + L::BAR_OFF;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (L::NS + s); };
+    const uint32_t b1 = bars + 16u * L::NS;
+    auto q_full = [&](int x) { return b1 + 8u * x; };
+    auto q_empty = [&](int x) { return b1 + 8u * (2 + x); };
+    auto s_full = [&](int x) { return b1 + 8u * (4 + x); };
+    auto p_full = [&](int x) { return b1 + 8u * (6 + x); };
+    auto o_full = [&](int x) { return b1 + 8u * (8 + x); };
+
+    if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
+        if (tid == 0) atomicExch(p.err, 1);
+        return;
     }
-    for (int64_t j = j0; j < j1; ++j) {
-        const int64_t page = d.block_table[r * d.table_stride + j / d.page_size], off = j % d.page_size;
-        if (page < 0 || page >= d.n_pages) continue;
-        const T* k = static_cast<const T*>(d.k_pool) + page * d.kp_sp + hk * d.kp_sh + off * d.kp_st + lane * E;
-        const T* v = static_cast<const T*>(d.v_pool) + page * d.vp_sp + hk * d.vp_sh + off * d.vp_st + lane * E;
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += q[e] * Elem<DT>::to_f(k[e]);
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-        s *= (float)d.sm_scale;
-        const float mn = fmaxf(m, s);
-        const float a = m == mn ? 1.f : expf(m - mn), b = expf(s - mn);
-        m = mn;
-        l = l * a + b;
-        for (int e = 0; e < E; ++e) acc[e] = acc[e] * a + b * Elem<DT>::to_f(v[e]);
+    if (tid == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < L::NS; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(q_full(x), 1);
+            mbar_init(q_empty(x), 1);
+            mbar_init(s_full(x), 1);
+            mbar_init(p_full(x), 4);
+            mbar_init(o_full(x), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        p.rec[cta * 4] = make_int4(0, 0, 0, 0);
+        p.rec[cta * 4 + 2] = make_int4(0, 0, 0, 0);
     }
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    for (int e = 0; e < E; ++e)
-        static_cast<T*>(d.out)[t * d.o_st + h * d.o_sh + lane * E + e] = Elem<DT>::from_f(acc[e] * inv);
-    if (d.lse && lane == 0) d.lse[w] = m + logf(l);
+    if (warp == 9) {
+        tc_alloc(sb + L::MISC_OFF, 512);
+        tc_relinquish();
+    }
+
+    // ---- this CTA's range of work: scan of the requests' costs ----
+    Walk walk;
+    {
+        int64_t* sums = reinterpret_cast<int64_t*>(smem + L::RING_OFF);        // [10] per warp
+        int64_t* found = sums + 16;                                            // b, h, start, y, i, pos
+        const int per = (p.R + kCaThreads - 1) / kCaThreads;
+        const int r0 = min(p.R, tid * per), r1 = min(p.R, r0 + per);
+        int64_t mine = 0;
+        for (int b = r0; b < r1; ++b) {
+            const Req r = load_req(p, b);
+            mine += tiles_cost(p, r, tiles_of(p, r));
+        }
+        int64_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t a = __shfl_up_sync(~0u, incl, o);
+            if (lane >= o) incl += a;
+        }
+        if (lane == 31) sums[warp] = incl;
+        __syncthreads();
+        int64_t before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < kCaThreads / 32; ++w) {
+            if (w == warp) before = all;
+            all += sums[w];
+        }
+        const int64_t W = all * p.Hkv;
+        const int64_t share = (W + kMinShare - 1) / kMinShare;
+        const int Ge = (int)min((int64_t)G, share);
+        const bool works = cta < Ge;
+        walk.x0 = works ? W * cta / Ge : 0;
+        walk.x1 = works ? W * (cta + 1) / Ge : 0;
+        int64_t at = (before + incl - mine) * p.Hkv;
+        if (works && walk.x0 >= at && walk.x0 < at + mine * p.Hkv) {
+            for (int b = r0; b < r1; ++b) {
+                const Req r = load_req(p, b);
+                const int64_t c = tiles_cost(p, r, tiles_of(p, r));
+                if (walk.x0 < at + c * p.Hkv) {
+                    const int64_t h = (walk.x0 - at) / c;
+                    found[0] = b;
+                    found[1] = h;
+                    found[2] = at + h * c;
+                    break;
+                }
+                at += c * p.Hkv;
+            }
+        }
+        __syncthreads();
+        walk.b = works ? (int)found[0] : 0;
+        walk.h = works ? (int)found[1] : 0;
+        walk.pos = works ? found[2] : 0;
+        if (works) {
+            walk.r = load_req(p, walk.b);
+            walk.nt = tiles_of(p, walk.r);
+            const int64_t y = walk.x0 - walk.pos;
+            for (int i = tid; i < walk.nt; i += kCaThreads) {
+                const int64_t c = tiles_cost(p, walk.r, i);
+                if (c <= y && y < tiles_cost(p, walk.r, i + 1)) {
+                    found[4] = i;
+                    found[5] = walk.pos + c;
+                }
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring is TMA's from here on
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        walk.i = works ? (int)found[4] : 0;
+        if (works) walk.pos = found[5];
+        __syncthreads();
+    }
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFF);
+    griddep_launch_dependents();
+    Seg s;
+
+    if (warp == 8) {
+        // ------------------------------ loads ------------------------------
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_k)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_v)) : "memory");
+        }
+        const int ppb = kBlk >> p.page_log2, page = 1 << p.page_log2;
+        const uint32_t q_bytes = 128u * (D / 64) * p.g * p.tq;
+        uint32_t q_uses[2] = {0, 0};
+        int flip = 0, stage = 0;
+        uint32_t phase = 0;
+        while (walk.next(p, s)) {
+            if (s.k1 == s.k0) continue;
+            const bool two = s.n > p.tq;
+            for (int x = two ? 0 : flip; x < (two ? 2 : flip + 1); ++x) {
+                ca_wait(q_empty(x), (q_uses[x] & 1u) ^ 1u, abort_flag, p.err);
+                ++q_uses[x];
+                if (lane == 0) {
+                    mbar_arrive_tx(q_full(x), q_bytes);
+                    const int t = s.r.q0 + s.t0 + (two ? x * p.tq : 0);
+                    for (int c = 0; c < D / 64; ++c)
+                        tma_load_3d(sb + L::Q_OFF + x * L::TILE + c * L::SUB, &tmap_q, c * 64, s.h * p.g, t, q_full(x));
+                }
+            }
+            if (!two) flip ^= 1;
+            // page ids, 32 entries at a time: this group and the next
+            const int32_t* row = p.block_table + s.b * p.table_stride;
+            const int n_pg = (s.r.kv + page - 1) >> p.page_log2;
+            auto entry = [&](int at) {
+                const int id = at < n_pg ? row[at] : p.n_pages;
+                return (uint32_t)id < (uint32_t)p.n_pages ? id : p.n_pages;   // beyond the pool: zeros
+            };
+            int base = s.k0 * ppb & ~31;
+            int cur = entry(base + lane), nxt = entry(base + 32 + lane);
+            for (int kb = s.k0; kb < s.k1; ++kb) {
+                if (kb * ppb >= base + 32) {
+                    base += 32;
+                    cur = nxt;
+                    nxt = entry(base + 32 + lane);
+                }
+                const int id = __shfl_sync(~0u, cur, (kb * ppb + (lane % ppb)) & 31);
+                for (int kv = 0; kv < 2; ++kv) {
+                    ca_wait(empty(stage), phase ^ 1u, abort_flag, p.err);
+                    if (lane == 0) mbar_arrive_tx(full(stage), L::TILE);
+                    __syncwarp();
+                    // lane = page of the block + ppb * sub-tile
+                    if (lane < ppb * (D / 64)) {
+                        const int pg = lane % ppb, c = lane / ppb;
+                        tma_load_4d(sb + L::RING_OFF + stage * L::TILE + c * L::SUB + ((pg * 128) << p.page_log2),
+                                    kv ? &tmap_v : &tmap_k, c * 64, 0, s.h, id, full(stage));
+                    }
+                    if (++stage == L::NS) stage = 0, phase ^= 1u;
+                }
+            }
+        }
+        // every copy has landed before the CTA may exit
+        for (int i = 0; i < L::NS; ++i) {
+            ca_wait(empty(stage), phase ^ 1u, abort_flag, p.err);
+            if (++stage == L::NS) stage = 0, phase ^= 1u;
+        }
+    } else if (warp == 9) {
+        // ------------------------------- MMA -------------------------------
+        if (lane == 0) {
+            constexpr uint32_t IQK = ca_idesc<DT>(kBlk, false), IPV = ca_idesc<DT>(D, true);
+            uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+            int flip = 0;
+            uint32_t ring = 0;   // blocks' stages consumed so far: K of block j at ring + 2 j, V one later
+            auto wait_stage = [&](uint32_t pos) {
+                ca_wait(full(pos % L::NS), (pos / L::NS) & 1u, abort_flag, p.err);
+                tc_fence_after();
+                return sb + L::RING_OFF + (pos % L::NS) * L::TILE;
+            };
+            auto qk = [&](int st, int qb, uint32_t kaddr) {
+                const uint32_t qaddr = sb + L::Q_OFF + qb * L::TILE;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    tc_mma_ss(tmem + kColS + 128 * st, tc_desc(qaddr + (ks >> 2) * L::SUB + (ks & 3) * 32, 16, 1024, 2),
+                              tc_desc(kaddr + (ks >> 2) * L::SUB + (ks & 3) * 32, 16, 1024, 2), IQK, ks > 0 ? 1u : 0u);
+                tc_commit(s_full(st));
+            };
+            auto pv = [&](int st, uint32_t vaddr, bool first) {
+                ca_wait(p_full(st), p_uses[st] & 1u, abort_flag, p.err);
+                ++p_uses[st];
+                tc_fence_after();
+#pragma unroll
+                for (int ks = 0; ks < kBlk / 16; ++ks)
+                    tc_mma_ts(tmem + kColO + D * st, tmem + kColS + 128 * st + 8 * ks,
+                              tc_desc(vaddr + ks * 2048, L::SUB, 1024, 2), IPV, (first && ks == 0) ? 0u : 1u);
+            };
+            while (walk.next(p, s)) {
+                const int nb = s.k1 - s.k0;
+                if (nb == 0) continue;
+                const bool two = s.n > p.tq;
+                const int q0 = two ? 0 : flip, q1 = two ? 1 : flip;   // Q buffers of the streams
+                for (int x = q0; x <= q1; ++x) {
+                    ca_wait(q_full(x), q_uses[x] & 1u, abort_flag, p.err);
+                    ++q_uses[x];
+                }
+                tc_fence_after();
+                if (!two) flip ^= 1;
+                auto kpos = [&](int j) { return ring + 2u * j; };
+                auto vpos = [&](int j) { return ring + 2u * j + 1u; };
+                auto release = [&](uint32_t pos) { tc_commit(empty(pos % L::NS)); };
+                auto q_done = [&](int j_last, int j) {
+                    if (j == j_last)
+                        for (int x = q0; x <= q1; ++x) tc_commit(q_empty(x));
+                };
+                if (two) {
+                    uint32_t ka = wait_stage(kpos(0));
+                    qk(0, q0, ka);
+                    qk(1, q1, ka);
+                    release(kpos(0));
+                    q_done(nb - 1, 0);
+                    for (int j = 0; j < nb; ++j) {
+                        const uint32_t va = wait_stage(vpos(j));
+                        pv(0, va, j == 0);
+                        if (j + 1 < nb) {
+                            ka = wait_stage(kpos(j + 1));
+                            qk(0, q0, ka);
+                        } else {
+                            tc_commit(o_full(0));
+                        }
+                        pv(1, va, j == 0);
+                        release(vpos(j));
+                        if (j + 1 < nb) {
+                            qk(1, q1, ka);
+                            release(kpos(j + 1));
+                            q_done(nb - 1, j + 1);
+                        } else {
+                            tc_commit(o_full(1));
+                        }
+                    }
+                } else {
+                    for (int j = 0; j < min(nb, 2); ++j) {
+                        qk(j, q0, wait_stage(kpos(j)));
+                        release(kpos(j));
+                        q_done(nb - 1, j);
+                    }
+                    for (int j = 0; j < nb; ++j) {
+                        const int st = j & 1;
+                        pv(st, wait_stage(vpos(j)), j < 2);
+                        release(vpos(j));
+                        if (j + 2 < nb) {
+                            qk(st, q0, wait_stage(kpos(j + 2)));
+                            release(kpos(j + 2));
+                            q_done(nb - 1, j + 2);
+                        } else {
+                            tc_commit(o_full(st));
+                        }
+                    }
+                }
+                ring += 2u * nb;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ----------------------------- softmax -----------------------------
+        const int st = warp / 4, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // this warp's 32 lanes of tensor memory
+        const uint32_t ts = tmem + lanes + kColS + 128 * st, to = tmem + lanes + kColO + D * st;
+        const float sl = p.scale_log2, lazy = kLazyMax / sl;
+        float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
+        const int tok = row / p.g, head = row % p.g;                  // token within the half tile
+        uint32_t s_uses = 0, o_uses = 0, ring = 0;
+        while (walk.next(p, s)) {
+            const int nb = s.k1 - s.k0;
+            const bool two = s.n > p.tq;
+            const int t = s.t0 + (two ? st * p.tq : 0) + tok;         // token within the request
+            const bool valid = tok < p.tq && t < s.t0 + s.n;
+            const int64_t orow = (int64_t)(s.r.q0 + t);
+            const int hq = s.h * p.g + head;
+            T* orow_p = static_cast<T*>(p.out) + orow * p.o_st + (int64_t)hq * p.o_sh;
+            if (nb == 0) {   // no key is visible
+                if (valid && (two || st == 0)) {
+                    for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(orow_p + c) = make_uint4(0u, 0u, 0u, 0u);
+                    if (p.lse) p.lse[orow * p.Hq + hq] = -INFINITY;
+                }
+                continue;
+            }
+            const bool warp_on = __any_sync(~0u, valid);
+            // keys of this row: [kmin, kend)
+            const int pos = s.r.off + t;
+            const int kend = p.causal ? min(pos + 1, s.r.kv) : s.r.kv;
+            const int kmin = p.window > 0 ? pos - p.window + 1 : 0;
+            // keys that every row of the half tile sees
+            const int first = s.r.off + s.t0 + (two ? st * p.tq : 0);
+            const int all_end = p.causal ? min(first + 1, s.r.kv) : s.r.kv;
+            const int all_min = p.window > 0 ? first + p.tq - p.window : 0;
+            float m = -INFINITY, l = 0.f;
+            const int step = two ? 1 : 2;
+            int blocks = 0;
+            for (int kb = s.k0 + (two ? 0 : st); kb < s.k1; kb += step, ++blocks) {
+                const bool ok = __all_sync(~0u, ca_wait(s_full(st), s_uses & 1u, abort_flag, p.err));
+                ++s_uses;
+                tc_fence_after();
+                if (warp_on && ok) {
+                    uint32_t x[128];
+                    tc_ld32(ts, x, 0);
+                    tc_ld32(ts + 32, x, 32);
+                    tc_ld32(ts + 64, x, 64);
+                    tc_ld32(ts + 96, x, 96);
+                    tc_wait_ld32(x, 0);
+                    tc_wait_ld32(x, 32);
+                    tc_wait_ld32(x, 64);
+                    tc_wait_ld32(x, 96);
+                    const int k0 = kb * kBlk;
+                    if (k0 + kBlk > all_end || k0 < all_min) {
+                        const int je = kend - k0, jm = kmin - k0;
+#pragma unroll
+                        for (int j = 0; j < 128; ++j)
+                            if (j >= je || j < jm) x[j] = 0xff800000u;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[c]);
+#pragma unroll
+                    for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j]));
+                    const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    const bool need = bm > m + lazy;
+                    if (__any_sync(~0u, need)) {
+                        const float mn = need ? bm : m;
+                        const float a = need ? ex2((m - mn) * sl) : 1.f;
+                        m = mn;
+                        l *= a;
+                        if (blocks > 0) {   // the output so far, in tensor memory, to the new maximum
+#pragma unroll
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                tc_ld16(to + c, o);
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+                                tc_st16(to + c, o);
+                            }
+                        }
+                    }
+                    const float off = m == -INFINITY ? 0.f : m * sl;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t w[64];
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) {
+                        const float a = ex2(fmaf(__uint_as_float(x[2 * j]), sl, -off));
+                        const float b = ex2(fmaf(__uint_as_float(x[2 * j + 1]), sl, -off));
+                        sum[(2 * j) & 3] += a;
+                        sum[(2 * j + 1) & 3] += b;
+                        w[j] = pack2<DT>(a, b);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_st32(ts, w, 0);
+                    tc_st32(ts + 32, w, 32);
+                    tc_wait_st();
+                }
+                // keys past the end of the cache: their V rows (the rest of a page) may hold anything
+                if (kb * kBlk + kBlk > s.r.kv && (!two || st == 0)) {
+                    const uint32_t vp = ring + 2u * (kb - s.k0) + 1u;
+                    ca_wait(full(vp % L::NS), (vp / L::NS) & 1u, abort_flag, p.err);
+                    const int keep = s.r.kv - kb * kBlk;
+                    uint8_t* v = smem + L::RING_OFF + (vp % L::NS) * L::TILE;
+                    for (int i = row; i < (kBlk - keep) * (D / 8); i += 128) {
+                        const int r = keep + i / (D / 8), c = i % (D / 8);
+                        *reinterpret_cast<uint4*>(v + (c / 8) * L::SUB + r * 128 + (c % 8) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(st));
+            }
+            ring += 2u * nb;
+            if (blocks > 0) {
+                ca_wait(o_full(st), o_uses & 1u, abort_flag, p.err);
+                ++o_uses;
+            }
+            __syncwarp();
+            tc_fence_after();
+            // ---- this stream's rows, or both streams' halves of the channels ----
+            float e0 = 1.f, e1 = 0.f;   // factors of the outputs of streams 0 and 1
+            float mlog = m * sl;        // -inf while no key was seen
+            if (!two) {
+                ml[st * 128 + row] = make_float2(mlog, l);
+                tc_fence_before();
+                wg_bar(1, 256);
+                tc_fence_after();
+                const float2 a = ml[row], b = ml[128 + row];
+                mlog = fmaxf(a.x, b.x);
+                e0 = a.x == -INFINITY ? 0.f : ex2(a.x - mlog);
+                e1 = b.x == -INFINITY ? 0.f : ex2(b.x - mlog);
+                l = a.y * e0 + b.y * e1;
+            }
+            const bool whole = s.whole();
+            const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+            const int slot = cta * 2 + (s.k0 == s.lo_blk ? 1 : 0);
+            const int prow = two ? st * 128 + row : row;
+            const int c0 = two ? 0 : st * (D / 2), c1 = two ? D : c0 + D / 2;
+            if (warp_on) {
+                const uint32_t t0 = tmem + lanes + kColO + (two ? D * st : 0);
+                for (int c = c0; c < c1; c += 16) {
+                    uint32_t o[16];
+                    tc_ld16(t0 + c, o);
+                    float f[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(o[j]) * e0;
+                    if (!two && nb > 1) {
+                        tc_ld16(t0 + D + c, o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) f[j] += __uint_as_float(o[j]) * e1;
+                    }
+                    if (valid && whole) {
+                        uint32_t y[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
+                        *reinterpret_cast<uint4*>(orow_p + c) = make_uint4(y[0], y[1], y[2], y[3]);
+                        *reinterpret_cast<uint4*>(orow_p + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
+                    } else if (valid) {
+                        float4* o4 = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * 256 + prow) * D + c);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o4[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (valid && (two || st == 0)) {
+                if (!whole) p.part_ml[slot * 256 + prow] = make_float2(mlog, l);
+                else if (p.lse) p.lse[orow * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (mlog + __log2f(l));
+            }
+            if (tid == 0 && !whole) {
+                p.rec[slot * 2] = make_int4(1, s.k1, s.hi_blk, s.b);
+                p.rec[slot * 2 + 1] = make_int4(s.h, s.i, 0, 0);
+            }
+            tc_fence_before();
+            if (!two) wg_bar(1, 256);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tc_dealloc(tmem, 512);
+}
+
+// Joins the partial outputs of the tiles that cross a cut.  The tile begun in
+// CTA c's last segment continues as the first segment of c + 1, c + 2, ...
+// until its last key block.  16 threads per row, segments in order.
+template <int DT, int D>
+__global__ void __launch_bounds__(kJoinRows * 16) chunk_join_kernel(const ChunkParams p, int G) {
+    using T = typename Elem<DT>::T;
+    constexpr int E = D / 16;
+    griddep_wait();
+    const int c = blockIdx.x;
+    const int4 rec = p.rec[(c * 2 + 1) * 2];
+    if (!rec.x) return;
+    const int4 at = p.rec[(c * 2 + 1) * 2 + 1];
+    Req r = load_req(p, rec.w);
+    const int row = blockIdx.y * kJoinRows + threadIdx.x / 16, l16 = threadIdx.x % 16;
+    const int rows = min(2 * p.tq, r.qlen - at.y * 2 * p.tq) * p.g;   // tokens of the tile, all heads
+    const bool two = rows > p.tq * p.g;
+    // rows of the partials: half tiles start at 0 and 128
+    if (row >= 256) return;
+    const int half = row / 128, in_half = row % 128;
+    const int tok = in_half / p.g;
+    if (tok >= p.tq || (half && !two) || (half * p.tq + tok) * p.g >= rows) return;
+    // segments: c's last, then the first of the CTAs up to the one that ends the tile
+    int end = c;
+    for (int k1 = rec.y; k1 < rec.z && end + 1 < G;) {
+        ++end;
+        const int4 nx = p.rec[end * 4];
+        if (nx.x) k1 = nx.y;
+    }
+    auto slot_of = [&](int e) { return e == c ? c * 2 + 1 : e * 2; };
+    float m = -INFINITY;
+    auto has = [&](int e) { return e == c || p.rec[e * 4].x != 0; };
+    for (int e = c; e <= end; ++e)
+        if (has(e)) m = fmaxf(m, p.part_ml[slot_of(e) * 256 + row].x);
+    float l = 0.f, acc[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) acc[j] = 0.f;
+    for (int e = c; e <= end; ++e) {
+        if (!has(e)) continue;
+        const int64_t sr = (int64_t)slot_of(e) * 256 + row;
+        const float2 ml = p.part_ml[sr];
+        const float a = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        l += ml.y * a;
+        const float4* o4 = reinterpret_cast<const float4*>(p.part_o + sr * D + l16 * E);
+#pragma unroll
+        for (int j = 0; j < E / 4; ++j) {
+            const float4 v = o4[j];
+            acc[4 * j] += v.x * a;
+            acc[4 * j + 1] += v.y * a;
+            acc[4 * j + 2] += v.z * a;
+            acc[4 * j + 3] += v.w * a;
+        }
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    const int64_t t = (int64_t)r.q0 + at.y * 2 * p.tq + half * p.tq + tok;
+    const int hq = at.x * p.g + in_half % p.g;
+    uint32_t y[E / 2];
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) y[j] = pack2<DT>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    uint2* o = reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + l16 * E);
+#pragma unroll
+    for (int j = 0; j < E / 4; ++j) o[j] = make_uint2(y[2 * j], y[2 * j + 1]);
+    if (p.lse && l16 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+static PFN_cuTensorMapEncodeTiled_v12000 ca_encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
 }
 
 static int check_desc(const fade_chunk_desc* d) {
@@ -59,9 +812,53 @@ static int check_desc(const fade_chunk_desc* d) {
     if ((d->D != 64 && d->D != 128) || d->Hq / d->Hkv > 128) return FADE_ERR_UNSUPPORTED;
     if (d->page_size != 16 && d->page_size != 32 && d->page_size != 64 && d->page_size != 128)
         return FADE_ERR_UNSUPPORTED;
-    if (d->R > INT32_MAX / 2 || d->T > INT32_MAX / d->Hq || d->n_pages > INT32_MAX ||
-        d->table_width > INT32_MAX / d->page_size)
+    // 32-bit positions: sums of two lengths stay below 2^31
+    const int64_t most = 1LL << 29;
+    if (d->R > most || d->T > most || d->Hq > (1 << 20) || d->n_pages > INT32_MAX - 1 ||
+        d->table_width > most / d->page_size)
         return FADE_ERR_UNSUPPORTED;
+    return FADE_OK;
+}
+
+// [T, Hq, D] or [pages, heads, tokens, D] in 64-channel boxes, 128-byte swizzle
+static int make_map(CUtensorMap* m, int dtype, const void* base, int rank, const cuuint64_t* dims,
+                    const int64_t* strides, const cuuint32_t* box) {
+    auto enc = ca_encode_fn();
+    if (!enc) return FADE_ERR_CUDA;
+    cuuint64_t bytes[3];
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank - 1; ++i) {
+        if (strides[i] < 0) return FADE_ERR_INVALID_ARG;
+        bytes[i] = (cuuint64_t)strides[i] * 2;
+    }
+    const CUresult r = enc(m, dtype == FADE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                           rank, const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? FADE_OK : FADE_ERR_ALIGN;
+}
+
+static size_t ws_bytes_for(int G, int64_t D) {
+    return 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8 + (size_t)G * 2 * 256 * D * 4;
+}
+
+template <int DT, int D>
+static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const ChunkParams& p, int G,
+                        int slices, cudaStream_t st) {
+    auto k = chunk_attn_kernel<DT, D>;
+    FADE_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, CaLayout<D>::BYTES));
+    k<<<G, kCaThreads, CaLayout<D>::BYTES, st>>>(tq, tk, tv, p);
+    FADE_LAUNCH_CHECK();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(G, slices);
+    cfg.blockDim = dim3(kJoinRows * 16);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    FADE_CUDA_TRY(cudaLaunchKernelEx(&cfg, chunk_join_kernel<DT, D>, p, G));
     return FADE_OK;
 }
 
@@ -70,7 +867,9 @@ static int check_desc(const fade_chunk_desc* d) {
 using namespace fade;
 
 extern "C" size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d) {
-    return check_desc(d) == FADE_OK ? 256 : 0;
+    if (check_desc(d) != FADE_OK) return 0;
+    const int G = fade_sm_count();
+    return ws_bytes_for(G > 0 ? G : 148, d->D);
 }
 
 extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream) {
@@ -85,15 +884,55 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
         if (s % 8) return FADE_ERR_ALIGN;
     if (!aligned16(d->q) || !aligned16(d->out) || !aligned16(d->k_pool) || !aligned16(d->v_pool)) return FADE_ERR_ALIGN;
     if (!workspace || ws_bytes < fade_chunk_attn_workspace_size(d)) return FADE_ERR_WORKSPACE;
-    const unsigned grid = (unsigned)((d->T * d->Hq + 3) / 4);
-    cudaStream_t st = as_stream(stream);
-    if (d->dtype == FADE_F16) {
-        if (d->D == 64) chunk_attn_kernel<FADE_F16, 64><<<grid, 128, 0, st>>>(*d);
-        else chunk_attn_kernel<FADE_F16, 128><<<grid, 128, 0, st>>>(*d);
-    } else {
-        if (d->D == 64) chunk_attn_kernel<FADE_BF16, 64><<<grid, 128, 0, st>>>(*d);
-        else chunk_attn_kernel<FADE_BF16, 128><<<grid, 128, 0, st>>>(*d);
-    }
-    FADE_LAUNCH_CHECK();
-    return FADE_OK;
+    const int G = fade_sm_count();
+    if (G <= 0) return FADE_ERR_CUDA;
+    ChunkParams p = {};
+    p.block_table = d->block_table;
+    p.cu_q = d->cu_q;
+    p.kv_lens = d->kv_lens;
+    p.out = d->out;
+    p.lse = d->lse;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.err = reinterpret_cast<int*>(ws);
+    p.rec = reinterpret_cast<int4*>(ws + 256);
+    p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * 64);
+    p.part_o = reinterpret_cast<float*>(ws + 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8);
+    p.table_stride = d->table_stride;
+    p.o_st = d->o_st;
+    p.o_sh = d->o_sh;
+    p.R = (int)d->R;
+    p.T = (int)d->T;
+    p.Hq = (int)d->Hq;
+    p.Hkv = (int)d->Hkv;
+    p.g = p.Hq / p.Hkv;
+    p.tq = kHalf / p.g;
+    while ((1 << p.page_log2) < d->page_size) ++p.page_log2;
+    p.n_pages = (int)d->n_pages;
+    p.table_width = d->n_pages > 0 ? (int)d->table_width : 0;
+    p.causal = d->causal != 0;
+    p.window = d->window >= (1LL << 29) ? 0 : (int)d->window;   // as long as the longest cache: hides nothing
+    p.scale_log2 = (float)(d->sm_scale * 1.4426950408889634);
+    CUtensorMap tq, tk, tv;
+    const cuuint64_t qd[3] = {(cuuint64_t)d->D, (cuuint64_t)d->Hq, (cuuint64_t)d->T};
+    const int64_t qs[2] = {d->q_sh, d->q_st};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)p.g, (cuuint32_t)p.tq};
+    int st = make_map(&tq, (int)d->dtype, d->q, 3, qd, qs, qb);
+    if (st != FADE_OK) return st;
+    // without a pool every table entry lies beyond it; the maps then describe q's memory and read nothing
+    const void* kb = d->n_pages > 0 ? d->k_pool : d->q;
+    const void* vb = d->n_pages > 0 ? d->v_pool : d->q;
+    const cuuint64_t kd[4] = {(cuuint64_t)d->D, (cuuint64_t)d->page_size, (cuuint64_t)d->Hkv,
+                              (cuuint64_t)(d->n_pages > 0 ? d->n_pages : 1)};
+    const int64_t ks[3] = {d->kp_st, d->kp_sh, d->kp_sp}, vs[3] = {d->vp_st, d->vp_sh, d->vp_sp};
+    const cuuint32_t kbox[4] = {64, (cuuint32_t)d->page_size, 1, 1};
+    if ((st = make_map(&tk, (int)d->dtype, kb, 4, kd, ks, kbox)) != FADE_OK) return st;
+    if ((st = make_map(&tv, (int)d->dtype, vb, 4, kd, vs, kbox)) != FADE_OK) return st;
+    const int64_t most_rows = std::min<int64_t>(256, d->T > 256 ? 256 : d->T * p.g);
+    const int slices = (int)((d->T > p.tq ? 256 : most_rows) + kJoinRows - 1) / kJoinRows;
+    cudaStream_t s = as_stream(stream);
+    if (d->dtype == FADE_F16)
+        return d->D == 64 ? launch_chunk<FADE_F16, 64>(tq, tk, tv, p, G, slices, s)
+                          : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, slices, s);
+    return d->D == 64 ? launch_chunk<FADE_BF16, 64>(tq, tk, tv, p, G, slices, s)
+                      : launch_chunk<FADE_BF16, 128>(tq, tk, tv, p, G, slices, s);
 }
