@@ -27,7 +27,8 @@
 // joined by a second kernel.  So ragged batches, the causal triangle and few
 // long rows all fill the GPU alike, from lengths that only the device knows.
 //
-// Warps of a CTA: 0-3 and 4-7 softmax, 8 loads (TMA, one box per page), 9 MMA.
+// Warps of a CTA: 0-3 and 4-7 softmax, 8 loads (TMA, one box per page), 9 and
+// 11 MMA, 10 walks the tiles and posts the segments.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -42,12 +43,13 @@ namespace fade {
 
 constexpr int kBlk = 128;              // keys per block
 constexpr int kHalf = 128;             // rows of a half tile
-constexpr int kCaThreads = 320;
+constexpr int kCaThreads = 384;
 constexpr int kCaSmemMax = 232448;     // 227 KB
 constexpr int kTileCost = 128;         // fixed cost of a tile, in keys
 constexpr int kMinShare = 256;         // least work of a CTA, in keys: one block per stream
 constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the maximum is moved
 constexpr uint32_t kCaPolls = 1u << 22;
+constexpr uint32_t kSegPolls = 1u << 26;
 constexpr int kJoinRows = 8;           // rows per CTA of the joining kernel
 
 struct ChunkParams {
@@ -59,10 +61,10 @@ struct ChunkParams {
     int* err;
     int4* rec;          // [CTA][2][2]: partial segments (continued tile, begun tile)
     float2* part_ml;    // [CTA][2][256]: (maximum in the log2 domain, sum)
-    float* part_o;      // [CTA][2][256][D]
+    float4* part_o;     // [CTA][2][D / 4][256]
     int64_t table_stride, o_st, o_sh;
-    int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window;
-    float scale_log2;
+    int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32;
+    float scale_log2, lazy;   // lazy: how far a score may exceed the running maximum
 };
 
 // ---------------------------------------------------------------------------
@@ -99,30 +101,33 @@ __device__ __forceinline__ int tiles_of(const ChunkParams& p, const Req& r) {
     return (r.qlen + 2 * p.tq - 1) / (2 * p.tq);
 }
 
-// A tile, or the part of its key blocks that a CTA works on.
-struct Seg {
-    Req r;
-    int b, h, i, n;            // request, kv head, tile, its tokens
-    int t0;                    // its first token, within the request
-    int lo_blk, hi_blk;        // key blocks of the tile
-    int k0, k1;                // of this segment
-    __device__ bool whole() const { return k0 == lo_blk && k1 == hi_blk; }
+// A tile, or the part of its key blocks that a CTA works on; handed from the
+// walking warp to the others through shared memory.
+struct __align__(16) Seg {
+    int k0, k1;                // key blocks of this segment
+    int n;                     // tokens of the tile; 0 ends the list
+    int kv;                    // keys of the request
+    int tok, pos;              // first token (in q) and its position
+    int b, h;                  // request, kv head
+    int lo_blk, hi_blk, i;     // key blocks of the whole tile, its index
+    int unused;
 };
+constexpr int kSegSlots = 4;
 
 struct Walk {
     Req r;
     int b, h, i, nt;
-    int64_t pos, x1, x0;       // cost position of the tile, range of the CTA
+    int64_t pos, x0, x1;       // cost position of the tile, range of the CTA
 
     __device__ __forceinline__ bool next(const ChunkParams& p, Seg& s) {
         while (pos < x1) {
-            const int t = 2 * p.tq;
-            s.r = r;
+            const int t = 2 * p.tq, t0 = i * t;
+            s.n = min(t, r.qlen - t0);
+            s.kv = r.kv;
+            s.tok = r.q0 + t0, s.pos = r.off + t0;
             s.b = b, s.h = h, s.i = i;
-            s.t0 = i * t;
-            s.n = min(t, r.qlen - s.t0);
-            const int hi = p.causal ? min(max(r.off + s.t0 + s.n, 0), r.kv) : r.kv;
-            const int lo = p.window > 0 ? min(max(r.off + s.t0 - p.window + 1, 0), hi) : 0;
+            const int hi = p.causal ? min(max(s.pos + s.n, 0), r.kv) : r.kv;
+            const int lo = p.window > 0 ? min(max(s.pos - p.window + 1, 0), hi) : 0;
             s.lo_blk = lo / kBlk;
             s.hi_blk = hi > lo ? (hi + kBlk - 1) / kBlk : s.lo_blk;
             const int cost = kTileCost + hi - lo;
@@ -225,12 +230,49 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&v)[N], 
         "r"(v[o + 26]), "r"(v[o + 27]), "r"(v[o + 28]), "r"(v[o + 29]), "r"(v[o + 30]), "r"(v[o + 31])
         : "memory");
 }
+// pairs of fp32 values in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     if (DT == FADE_BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+// 32 bytes of a row: one store where every row is 32-byte aligned (a warp stores 32 rows, each its own cache line,
+// and the lines, not the bytes, bound it)
+template <int N>
+__device__ __forceinline__ void st_row32(void* dst, const uint32_t (&v)[N], int o, int aligned) {
+    if (aligned) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[o]), "r"(v[o + 1]),
+                     "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+                     : "memory");
+    } else {
+        static_cast<uint4*>(dst)[0] = make_uint4(v[o], v[o + 1], v[o + 2], v[o + 3]);
+        static_cast<uint4*>(dst)[1] = make_uint4(v[o + 4], v[o + 5], v[o + 6], v[o + 7]);
+    }
 }
 // Instruction descriptor, kind::f16: f32 accumulator, A and B in the model dtype, M = 128, N columns;
 // b_mn: B is MN-major.
@@ -239,10 +281,6 @@ __host__ __device__ constexpr uint32_t ca_idesc(int n, bool b_mn) {
     return (1u << 4) | ((DT == FADE_BF16 ? 1u : 0u) << 7) | ((DT == FADE_BF16 ? 1u : 0u) << 10) |
            ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void wg_bar(int id, int threads) {
-    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 // Shared memory.  Q, K and V tiles are 128 rows of 128 bytes (64 channels) in
 // the 128-byte swizzle, one such sub-tile per 64 channels.
 template <int D>
@@ -254,9 +292,11 @@ struct CaLayout {
     static constexpr int NS = D == 128 ? 5 : 11;           // ring stages, one K or V block each
     static constexpr int ML_OFF = RING_OFF + NS * TILE;    // (m, l) of both streams
     static constexpr int BAR_OFF = ML_OFF + 2 * 128 * 8;
-    static constexpr int N_BARS = 2 * NS + 10;
+    static constexpr int N_BARS = 2 * NS + 21 + 2 * kSegSlots;
     static constexpr int MISC_OFF = BAR_OFF + 8 * N_BARS;  // tensor-memory slot, abort flag
-    static constexpr int BYTES = MISC_OFF + 16;
+    static constexpr int SEG_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
+    static constexpr int SUM_OFF = SEG_OFF + kSegSlots * (int)sizeof(Seg);   // costs per warp
+    static constexpr int BYTES = SUM_OFF + kCaThreads / 32 * 8;
     static_assert(BYTES <= kCaSmemMax, "chunk attention shared memory over the per-CTA limit");
 };
 constexpr int kColS = 0;      // two score tiles of 128 columns; the weights overlay the first 64 of each
@@ -270,7 +310,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     using T = typename Elem<DT>::T;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sb = smem_u32(smem);
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int tid = threadIdx.x, lane = tid % 32;
+    const int warp = __shfl_sync(~0u, tid / 32, 0);   // known to be the same for the whole warp
     const int cta = blockIdx.x, G = gridDim.x;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 8);
     const uint32_t bars = sb + L::BAR_OFF;
@@ -282,6 +323,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     auto s_full = [&](int x) { return b1 + 8u * (4 + x); };
     auto p_full = [&](int x) { return b1 + 8u * (6 + x); };
     auto o_full = [&](int x) { return b1 + 8u * (8 + x); };
+    auto seg_full = [&](int x) { return b1 + 8u * (10 + x); };
+    auto seg_empty = [&](int x) { return b1 + 8u * (10 + kSegSlots + x); };
+    const uint32_t both = b1 + 8u * (10 + 2 * kSegSlots);   // the softmax warps meet
+    auto h_full = [&](int x) { return b1 + 8u * (11 + 2 * kSegSlots + x); };   // weights of the block's first half
+    auto turn = [&](int x, int w) { return b1 + 8u * (13 + 2 * kSegSlots + 4 * x + w); };   // warp w of stream x may take exponentials
 
     if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
         if (tid == 0) atomicExch(p.err, 1);
@@ -291,14 +337,21 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         *abort_flag = 0;
         for (int s = 0; s < L::NS; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+            mbar_init(empty(s), 2);
         }
         for (int x = 0; x < 2; ++x) {
             mbar_init(q_full(x), 1);
-            mbar_init(q_empty(x), 1);
+            mbar_init(q_empty(x), 2);
             mbar_init(s_full(x), 1);
             mbar_init(p_full(x), 4);
+            mbar_init(h_full(x), 4);
             mbar_init(o_full(x), 1);
+        }
+        mbar_init(both, 8);
+        for (int i = 0; i < 8; ++i) mbar_init(turn(i / 4, i % 4), 1);
+        for (int x = 0; x < kSegSlots; ++x) {
+            mbar_init(seg_full(x), 1);
+            mbar_init(seg_empty(x), 11);   // loads, two MMA and eight softmax warps
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         p.rec[cta * 4] = make_int4(0, 0, 0, 0);
@@ -309,301 +362,382 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         tc_relinquish();
     }
 
-    // ---- this CTA's range of work: scan of the requests' costs ----
-    Walk walk;
-    {
-        int64_t* sums = reinterpret_cast<int64_t*>(smem + L::RING_OFF);        // [10] per warp
-        int64_t* found = sums + 16;                                            // b, h, start, y, i, pos
-        const int per = (p.R + kCaThreads - 1) / kCaThreads;
-        const int r0 = min(p.R, tid * per), r1 = min(p.R, r0 + per);
-        int64_t mine = 0;
-        for (int b = r0; b < r1; ++b) {
+    // ---- costs of the requests, summed per warp (the walking warp finds this CTA's share) ----
+    int64_t* sums = reinterpret_cast<int64_t*>(smem + L::SUM_OFF);
+    const int per = (p.R + kCaThreads - 1) / kCaThreads;   // requests of a thread
+    auto cost_of = [&](int first, int n) {
+        int64_t c = 0;
+        for (int b = first; b < min(first + n, p.R); ++b) {
             const Req r = load_req(p, b);
-            mine += tiles_cost(p, r, tiles_of(p, r));
+            c += tiles_cost(p, r, tiles_of(p, r));
         }
-        int64_t incl = mine;
+        return c;
+    };
+    {
+        int64_t c = cost_of(tid * per, per);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t a = __shfl_up_sync(~0u, incl, o);
-            if (lane >= o) incl += a;
-        }
-        if (lane == 31) sums[warp] = incl;
-        __syncthreads();
-        int64_t before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < kCaThreads / 32; ++w) {
-            if (w == warp) before = all;
-            all += sums[w];
-        }
-        const int64_t W = all * p.Hkv;
-        const int64_t share = (W + kMinShare - 1) / kMinShare;
-        const int Ge = (int)min((int64_t)G, share);
-        const bool works = cta < Ge;
-        walk.x0 = works ? W * cta / Ge : 0;
-        walk.x1 = works ? W * (cta + 1) / Ge : 0;
-        int64_t at = (before + incl - mine) * p.Hkv;
-        if (works && walk.x0 >= at && walk.x0 < at + mine * p.Hkv) {
-            for (int b = r0; b < r1; ++b) {
-                const Req r = load_req(p, b);
-                const int64_t c = tiles_cost(p, r, tiles_of(p, r));
-                if (walk.x0 < at + c * p.Hkv) {
-                    const int64_t h = (walk.x0 - at) / c;
-                    found[0] = b;
-                    found[1] = h;
-                    found[2] = at + h * c;
-                    break;
-                }
-                at += c * p.Hkv;
-            }
-        }
-        __syncthreads();
-        walk.b = works ? (int)found[0] : 0;
-        walk.h = works ? (int)found[1] : 0;
-        walk.pos = works ? found[2] : 0;
-        if (works) {
-            walk.r = load_req(p, walk.b);
-            walk.nt = tiles_of(p, walk.r);
-            const int64_t y = walk.x0 - walk.pos;
-            for (int i = tid; i < walk.nt; i += kCaThreads) {
-                const int64_t c = tiles_cost(p, walk.r, i);
-                if (c <= y && y < tiles_cost(p, walk.r, i + 1)) {
-                    found[4] = i;
-                    found[5] = walk.pos + c;
-                }
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // the ring is TMA's from here on
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        walk.i = works ? (int)found[4] : 0;
-        if (works) walk.pos = found[5];
-        __syncthreads();
+        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(~0u, c, o);
+        if (lane == 0) sums[warp] = c;
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + L::MISC_OFF);
     griddep_launch_dependents();
+    Seg* segs = reinterpret_cast<Seg*>(smem + L::SEG_OFF);
     Seg s;
+    int seg = 0;
+    uint32_t seg_phase = 0;
+    // the next posted segment; every lane reads it, one says so
+    auto next_seg = [&] {
+        const bool ok = ca_wait(seg_full(seg), seg_phase, abort_flag, p.err);
+        s = segs[seg];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(seg_empty(seg));
+        if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
+        return ok && s.n > 0;
+    };
 
-    if (warp == 8) {
-        // ------------------------------ loads ------------------------------
-        if (lane == 0) {
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_k)) : "memory");
-            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_v)) : "memory");
-        }
-        const int ppb = kBlk >> p.page_log2, page = 1 << p.page_log2;
-        const uint32_t q_bytes = 128u * (D / 64) * p.g * p.tq;
-        uint32_t q_uses[2] = {0, 0};
-        int flip = 0, stage = 0;
-        uint32_t phase = 0;
-        while (walk.next(p, s)) {
-            if (s.k1 == s.k0) continue;
-            const bool two = s.n > p.tq;
-            for (int x = two ? 0 : flip; x < (two ? 2 : flip + 1); ++x) {
-                ca_wait(q_empty(x), (q_uses[x] & 1u) ^ 1u, abort_flag, p.err);
-                ++q_uses[x];
-                if (lane == 0) {
-                    mbar_arrive_tx(q_full(x), q_bytes);
-                    const int t = s.r.q0 + s.t0 + (two ? x * p.tq : 0);
-                    for (int c = 0; c < D / 64; ++c)
-                        tma_load_3d(sb + L::Q_OFF + x * L::TILE + c * L::SUB, &tmap_q, c * 64, s.h * p.g, t, q_full(x));
-                }
+    // 384 threads x 168 registers at launch: 256 x 216 + 128 x 72 stay below that
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 8) {
+            // ---------------------------- loads ----------------------------
+            if (lane == 0) {
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_k)) : "memory");
+                asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_v)) : "memory");
             }
-            if (!two) flip ^= 1;
-            // page ids, 32 entries at a time: this group and the next
-            const int32_t* row = p.block_table + s.b * p.table_stride;
-            const int n_pg = (s.r.kv + page - 1) >> p.page_log2;
-            auto entry = [&](int at) {
-                const int id = at < n_pg ? row[at] : p.n_pages;
-                return (uint32_t)id < (uint32_t)p.n_pages ? id : p.n_pages;   // beyond the pool: zeros
-            };
-            int base = s.k0 * ppb & ~31;
-            int cur = entry(base + lane), nxt = entry(base + 32 + lane);
-            for (int kb = s.k0; kb < s.k1; ++kb) {
-                if (kb * ppb >= base + 32) {
-                    base += 32;
-                    cur = nxt;
-                    nxt = entry(base + 32 + lane);
-                }
-                const int id = __shfl_sync(~0u, cur, (kb * ppb + (lane % ppb)) & 31);
-                for (int kv = 0; kv < 2; ++kv) {
-                    ca_wait(empty(stage), phase ^ 1u, abort_flag, p.err);
-                    if (lane == 0) mbar_arrive_tx(full(stage), L::TILE);
-                    __syncwarp();
-                    // lane = page of the block + ppb * sub-tile
-                    if (lane < ppb * (D / 64)) {
-                        const int pg = lane % ppb, c = lane / ppb;
-                        tma_load_4d(sb + L::RING_OFF + stage * L::TILE + c * L::SUB + ((pg * 128) << p.page_log2),
-                                    kv ? &tmap_v : &tmap_k, c * 64, 0, s.h, id, full(stage));
+            const int ppb = kBlk >> p.page_log2;
+            // lane = page of the block + ppb * sub-tile
+            const int my_page = lane % ppb, my_sub = lane / ppb;
+            const uint32_t my_dst = sb + L::RING_OFF + my_sub * L::SUB + ((my_page * 128) << p.page_log2);
+            uint32_t q_phase = 3;   // bit x: parity to wait for on buffer x
+            int flip = 0, stage = 0;
+            uint32_t phase = 1;
+            while (next_seg()) {
+                if (s.k1 == s.k0) continue;
+                const bool two = s.n > p.tq;
+                for (int x = two ? 0 : flip; x < (two ? 2 : flip + 1); ++x) {
+                    ca_wait(q_empty(x), (q_phase >> x) & 1u, abort_flag, p.err);
+                    q_phase ^= 1u << x;
+                    if (lane == 0) {
+                        mbar_arrive_tx(q_full(x), 128u * (D / 64) * p.g * p.tq);
+                        for (int c = 0; c < D / 64; ++c)
+                            tma_load_3d(sb + L::Q_OFF + x * L::TILE + c * L::SUB, &tmap_q, c * 64, s.h * p.g,
+                                        s.tok + (two ? x * p.tq : 0), q_full(x));
                     }
-                    if (++stage == L::NS) stage = 0, phase ^= 1u;
+                }
+                if (!two) flip ^= 1;
+                // page ids, 32 entries at a time: this group and the next
+                const int32_t* row = p.block_table + s.b * p.table_stride;
+                const int n_pg = (s.kv + (1 << p.page_log2) - 1) >> p.page_log2;
+                auto entry = [&](int at) {
+                    const int id = at < n_pg ? row[at] : p.n_pages;
+                    return (uint32_t)id < (uint32_t)p.n_pages ? id : p.n_pages;   // beyond the pool: zeros
+                };
+                int base = s.k0 * ppb & ~31;
+                int cur = entry(base + lane), nxt = entry(base + 32 + lane);
+                for (int kb = s.k0; kb < s.k1; ++kb) {
+                    if (kb * ppb >= base + 32) {
+                        base += 32;
+                        cur = nxt;
+                        nxt = entry(base + 32 + lane);
+                    }
+                    const int id = __shfl_sync(~0u, cur, (kb * ppb + my_page) & 31);
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        ca_wait(empty(stage), phase, abort_flag, p.err);
+                        if (lane == 0) mbar_arrive_tx(full(stage), L::TILE);
+                        __syncwarp();
+                        if (my_sub < D / 64)
+                            tma_load_4d(my_dst + stage * L::TILE, kv ? &tmap_v : &tmap_k, my_sub * 64, 0, s.h, id,
+                                        full(stage));
+                        if (++stage == L::NS) stage = 0, phase ^= 1u;
+                    }
                 }
             }
-        }
-        // every copy has landed before the CTA may exit
-        for (int i = 0; i < L::NS; ++i) {
-            ca_wait(empty(stage), phase ^ 1u, abort_flag, p.err);
-            if (++stage == L::NS) stage = 0, phase ^= 1u;
-        }
-    } else if (warp == 9) {
-        // ------------------------------- MMA -------------------------------
-        if (lane == 0) {
+            // every copy has landed before the CTA may exit
+            for (int i = 0; i < L::NS; ++i) {
+                ca_wait(empty(stage), phase, abort_flag, p.err);
+                if (++stage == L::NS) stage = 0, phase ^= 1u;
+            }
+        } else if (warp == 9 || warp == 11) {
+            // ---------------------- MMA, a warp per stream ----------------------
+            // Waits and commits take a warp about as long as half of a block's
+            // MMAs, so each stream has its own.  The whole warp walks the loop
+            // (addresses and descriptors stay in uniform registers), one lane
+            // issues.  Both warps go through every fill of every buffer, also
+            // where only the other one uses it (two arrivals free a buffer):
+            // a warp that skipped fills could mistake one for another.
+            const int st = warp == 9 ? 0 : 1;
+            const bool lead = elect_one();
             constexpr uint32_t IQK = ca_idesc<DT>(kBlk, false), IPV = ca_idesc<DT>(D, true);
-            uint32_t q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-            int flip = 0;
-            uint32_t ring = 0;   // blocks' stages consumed so far: K of block j at ring + 2 j, V one later
-            auto wait_stage = [&](uint32_t pos) {
-                ca_wait(full(pos % L::NS), (pos / L::NS) & 1u, abort_flag, p.err);
-                tc_fence_after();
-                return sb + L::RING_OFF + (pos % L::NS) * L::TILE;
+            const uint64_t q_desc = tc_desc(sb + L::Q_OFF, 16, 1024, 2);
+            const uint64_t k_desc = tc_desc(sb + L::RING_OFF, 16, 1024, 2);
+            const uint64_t v_desc = tc_desc(sb + L::RING_OFF, L::SUB, 1024, 2);
+            const uint32_t ts = tmem + kColS + 128 * st, to = tmem + kColO + D * st;
+            uint32_t q_phase = 0, p_phase = 0;   // bit x of q_phase: parity to wait for on buffer x
+            int flip = 0, stage = 0;             // next ring stage: K, V, K, V, ... of the blocks
+            uint32_t phase = 0;
+            auto landed = [&] { ca_wait(full(stage), phase, abort_flag, p.err); };
+            auto advance = [&] {
+                if (++stage == L::NS) stage = 0, phase ^= 1u;
             };
-            auto qk = [&](int st, int qb, uint32_t kaddr) {
-                const uint32_t qaddr = sb + L::Q_OFF + qb * L::TILE;
-#pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks)
-                    tc_mma_ss(tmem + kColS + 128 * st, tc_desc(qaddr + (ks >> 2) * L::SUB + (ks & 3) * 32, 16, 1024, 2),
-                              tc_desc(kaddr + (ks >> 2) * L::SUB + (ks & 3) * 32, 16, 1024, 2), IQK, ks > 0 ? 1u : 0u);
-                tc_commit(s_full(st));
+            auto pass = [&] {   // a block of the other stream
+                for (int i = 0; i < 2; ++i) {
+                    landed();
+                    if (lead) mbar_arrive(empty(stage));
+                    advance();
+                }
+                __syncwarp();
             };
-            auto pv = [&](int st, uint32_t vaddr, bool first) {
-                ca_wait(p_full(st), p_uses[st] & 1u, abort_flag, p.err);
-                ++p_uses[st];
-                tc_fence_after();
-#pragma unroll
-                for (int ks = 0; ks < kBlk / 16; ++ks)
-                    tc_mma_ts(tmem + kColO + D * st, tmem + kColS + 128 * st + 8 * ks,
-                              tc_desc(vaddr + ks * 2048, L::SUB, 1024, 2), IPV, (first && ks == 0) ? 0u : 1u);
-            };
-            while (walk.next(p, s)) {
+            while (next_seg()) {
                 const int nb = s.k1 - s.k0;
                 if (nb == 0) continue;
                 const bool two = s.n > p.tq;
-                const int q0 = two ? 0 : flip, q1 = two ? 1 : flip;   // Q buffers of the streams
-                for (int x = q0; x <= q1; ++x) {
-                    ca_wait(q_full(x), q_uses[x] & 1u, abort_flag, p.err);
-                    ++q_uses[x];
-                }
-                tc_fence_after();
+                if (two || flip == 0) ca_wait(q_full(0), q_phase & 1u, abort_flag, p.err);
+                if (two || flip == 1) ca_wait(q_full(1), q_phase >> 1, abort_flag, p.err);
+                const int x = two ? st : flip;   // Q buffer
+                q_phase ^= two ? 3u : 1u << flip;
                 if (!two) flip ^= 1;
-                auto kpos = [&](int j) { return ring + 2u * j; };
-                auto vpos = [&](int j) { return ring + 2u * j + 1u; };
-                auto release = [&](uint32_t pos) { tc_commit(empty(pos % L::NS)); };
-                auto q_done = [&](int j_last, int j) {
-                    if (j == j_last)
-                        for (int x = q0; x <= q1; ++x) tc_commit(q_empty(x));
+                const int mine = two ? nb : (nb + 1 - st) / 2;
+                if (lead && two) mbar_arrive(q_empty(st ^ 1));
+                if (lead && mine == 0) mbar_arrive(q_empty(x));
+                const uint64_t a = q_desc + (uint32_t)(x * (L::TILE >> 4));
+                auto scores = [&](bool last) {   // of the block whose K is next in the ring
+                    const uint64_t b = k_desc + (uint32_t)(stage * (L::TILE >> 4));
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint32_t o = (i >> 2) * (L::SUB >> 4) + (i & 3) * 2;
+                        tc_mma_ss(ts, a + o, b + o, IQK, i > 0 ? 1u : 0u);
+                    }
+                    tc_commit(s_full(st));
+                    tc_commit(empty(stage));
+                    if (last) tc_commit(q_empty(x));
                 };
-                if (two) {
-                    uint32_t ka = wait_stage(kpos(0));
-                    qk(0, q0, ka);
-                    qk(1, q1, ka);
-                    release(kpos(0));
-                    q_done(nb - 1, 0);
-                    for (int j = 0; j < nb; ++j) {
-                        const uint32_t va = wait_stage(vpos(j));
-                        pv(0, va, j == 0);
-                        if (j + 1 < nb) {
-                            ka = wait_stage(kpos(j + 1));
-                            qk(0, q0, ka);
-                        } else {
-                            tc_commit(o_full(0));
-                        }
-                        pv(1, va, j == 0);
-                        release(vpos(j));
-                        if (j + 1 < nb) {
-                            qk(1, q1, ka);
-                            release(kpos(j + 1));
-                            q_done(nb - 1, j + 1);
-                        } else {
-                            tc_commit(o_full(1));
-                        }
+                if (!two && st == 1) pass();
+                if (mine > 0) {
+                    landed();
+                    tc_fence_after();
+                    if (lead) scores(mine == 1);
+                    __syncwarp();
+                    advance();
+                }
+                for (int j = 0; j < mine; ++j) {
+                    const bool more = j + 1 < mine, now = two && more;   // the next scores follow at once
+                    landed();
+                    const uint64_t b = v_desc + (uint32_t)(stage * (L::TILE >> 4));
+                    const uint32_t v_empty = empty(stage);
+                    advance();
+                    if (now) landed();
+                    ca_wait(h_full(st), p_phase, abort_flag, p.err);
+                    tc_fence_after();
+                    if (lead) {
+                        tc_mma_ts(to, ts, b, IPV, j > 0 ? 1u : 0u);
+#pragma unroll
+                        for (int i = 1; i < kBlk / 32; ++i) tc_mma_ts(to, ts + 8 * i, b + (uint32_t)(i * 128), IPV, 1u);
                     }
-                } else {
-                    for (int j = 0; j < min(nb, 2); ++j) {
-                        qk(j, q0, wait_stage(kpos(j)));
-                        release(kpos(j));
-                        q_done(nb - 1, j);
+                    __syncwarp();
+                    ca_wait(p_full(st), p_phase, abort_flag, p.err);
+                    p_phase ^= 1u;
+                    tc_fence_after();
+                    if (lead) {
+#pragma unroll
+                        for (int i = kBlk / 32; i < kBlk / 16; ++i)
+                            tc_mma_ts(to, ts + 8 * i, b + (uint32_t)(i * 128), IPV, 1u);
+                        if (now) scores(j + 2 == mine);
+                        if (!more) tc_commit(o_full(st));
+                        tc_commit(v_empty);
                     }
-                    for (int j = 0; j < nb; ++j) {
-                        const int st = j & 1;
-                        pv(st, wait_stage(vpos(j)), j < 2);
-                        release(vpos(j));
-                        if (j + 2 < nb) {
-                            qk(st, q0, wait_stage(kpos(j + 2)));
-                            release(kpos(j + 2));
-                            q_done(nb - 1, j + 2);
-                        } else {
-                            tc_commit(o_full(st));
+                    __syncwarp();
+                    if (now) advance();
+                    if (!two) {
+                        if (2 * j + st + 1 < nb) pass();
+                        if (more) {
+                            landed();
+                            tc_fence_after();
+                            if (lead) scores(j + 2 == mine);
+                            __syncwarp();
+                            advance();
                         }
                     }
                 }
-                ring += 2u * nb;
             }
+        } else if (warp == 10) {
+            // ------------------------ tiles, in order ------------------------
+            // Range of this CTA: [x0, x1) of the total cost W, of which the
+            // first CTAs take one more when it does not divide.
+            Walk walk;
+            int64_t W = 0;
+#pragma unroll
+            for (int w = 0; w < kCaThreads / 32; ++w) W += sums[w];
+            W *= p.Hkv;
+            const int n_cta = (int)min((int64_t)G, (W + kMinShare - 1) / kMinShare);
+            const int64_t each = n_cta > 0 ? W / n_cta : 0;
+            const int rest = (int)(W - each * n_cta);
+            walk.x0 = cta < n_cta ? each * cta + min(cta, rest) : 0;
+            walk.x1 = cta < n_cta ? walk.x0 + each + (cta < rest ? 1 : 0) : 0;
+            walk.pos = 0;
+            if (cta < n_cta) {
+                // the warp's, the lane's, the request and the tile that x0 lies in
+                int64_t at = 0;
+                int w = 0;
+                for (; w + 1 < kCaThreads / 32 && walk.x0 >= at + sums[w] * p.Hkv; ++w) at += sums[w] * p.Hkv;
+                const int64_t mine = cost_of((w * 32 + lane) * per, per) * p.Hkv;
+                int64_t incl = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t v = __shfl_up_sync(~0u, incl, o);
+                    if (lane >= o) incl += v;
+                }
+                const int who = __ffs(__ballot_sync(~0u, walk.x0 < at + incl)) - 1;
+                at += __shfl_sync(~0u, incl - mine, who);
+                walk.b = (w * 32 + who) * per;
+                int64_t c;
+                for (;; ++walk.b) {
+                    walk.r = load_req(p, walk.b);
+                    walk.nt = tiles_of(p, walk.r);
+                    c = tiles_cost(p, walk.r, walk.nt);
+                    if (walk.x0 < at + c * p.Hkv || walk.b + 1 >= p.R) break;
+                    at += c * p.Hkv;
+                }
+                // a kv head's tiles cost c
+                walk.h = 0;
+                while (walk.h + 1 < p.Hkv && walk.x0 >= at + c) at += c, ++walk.h;
+                walk.i = 0;
+                for (int span = walk.nt; span > 1;) {   // 32 parts of the remaining tiles
+                    const int step = (span + 31) / 32, i = walk.i + lane * step;
+                    const bool below = lane * step < span && at + tiles_cost(p, walk.r, i) <= walk.x0;
+                    const int k = __popc(__ballot_sync(~0u, below)) - 1;
+                    span = min(step, span - k * step);
+                    walk.i += k * step;
+                }
+                walk.pos = at + tiles_cost(p, walk.r, walk.i);
+            }
+            if (lane == 0) {
+                bool more = true;
+                while (more) {
+                    more = walk.next(p, s);
+                    if (!more) s.n = 0;
+                    // a segment may take long: look for a free slot now and then
+                    for (uint32_t i = 0; i < kSegPolls && !mbar_try_wait(seg_empty(seg), seg_phase ^ 1u); ++i) {
+                        if (*abort_flag) break;
+                        if (i + 1 == kSegPolls) *abort_flag = 1, atomicExch(p.err, 1);
+                        __nanosleep(200);
+                    }
+                    segs[seg] = s;
+                    mbar_arrive(seg_full(seg));
+                    if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
+                }
+            }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ----------------------------- softmax -----------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int st = warp / 4, row = tid & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;            // this warp's 32 lanes of tensor memory
         const uint32_t ts = tmem + lanes + kColS + 128 * st, to = tmem + lanes + kColO + D * st;
-        const float sl = p.scale_log2, lazy = kLazyMax / sl;
+        const float sl = p.scale_log2;
         float2* ml = reinterpret_cast<float2*>(smem + L::ML_OFF);
-        const int tok = row / p.g, head = row % p.g;                  // token within the half tile
-        uint32_t s_uses = 0, o_uses = 0, ring = 0;
-        while (walk.next(p, s)) {
-            const int nb = s.k1 - s.k0;
-            const bool two = s.n > p.tq;
-            const int t = s.t0 + (two ? st * p.tq : 0) + tok;         // token within the request
-            const bool valid = tok < p.tq && t < s.t0 + s.n;
-            const int64_t orow = (int64_t)(s.r.q0 + t);
-            const int hq = s.h * p.g + head;
-            T* orow_p = static_cast<T*>(p.out) + orow * p.o_st + (int64_t)hq * p.o_sh;
-            if (nb == 0) {   // no key is visible
-                if (valid && (two || st == 0)) {
-                    for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(orow_p + c) = make_uint4(0u, 0u, 0u, 0u);
-                    if (p.lse) p.lse[orow * p.Hq + hq] = -INFINITY;
-                }
-                continue;
-            }
+        const int tok = row / p.g;                                    // token within the half tile
+        uint32_t s_phase = 0, o_phase = 0, ring = 0, meetings = 0, turn_phase = st ^ 1;
+        const uint32_t my_turn = turn(st, warp & 3), their_turn = turn(st ^ 1, warp & 3);
+        auto meet = [&] {   // a bounded wait, so that no warp is left behind when another gave up
+            __syncwarp();
+            if (lane == 0) mbar_arrive(both);
+            ca_wait(both, meetings & 1u, abort_flag, p.err);
+            ++meetings;
+            __syncwarp();
+        };
+        while (true) {
+            // the segment stays in its slot until this warp is through with it
+            ca_wait(seg_full(seg), seg_phase, abort_flag, p.err);
+            const Seg& g = segs[seg];
+            const int n = g.n;
+            if (n <= 0 || *abort_flag) break;
+            const bool two = n > p.tq;
+            const int k0 = g.k0, k1 = g.k1;
+            const int t = (two ? st * p.tq : 0) + tok;                // token within the tile
+            const bool valid = tok < p.tq && t < n;
             const bool warp_on = __any_sync(~0u, valid);
-            // keys of this row: [kmin, kend)
-            const int pos = s.r.off + t;
-            const int kend = p.causal ? min(pos + 1, s.r.kv) : s.r.kv;
-            const int kmin = p.window > 0 ? pos - p.window + 1 : 0;
-            // keys that every row of the half tile sees
-            const int first = s.r.off + s.t0 + (two ? st * p.tq : 0);
-            const int all_end = p.causal ? min(first + 1, s.r.kv) : s.r.kv;
-            const int all_min = p.window > 0 ? first + p.tq - p.window : 0;
             float m = -INFINITY, l = 0.f;
-            const int step = two ? 1 : 2;
             int blocks = 0;
-            for (int kb = s.k0 + (two ? 0 : st); kb < s.k1; kb += step, ++blocks) {
-                const bool ok = __all_sync(~0u, ca_wait(s_full(st), s_uses & 1u, abort_flag, p.err));
-                ++s_uses;
-                tc_fence_after();
-                if (warp_on && ok) {
+            {
+                // keys of this row: [kmin, kend); blocks that every row of the half tile sees whole: [free0, free1)
+                const int kv = g.kv, first = g.pos + (two ? st * p.tq : 0);
+                const int kend = p.causal ? min(first + tok + 1, kv) : kv;
+                const int kmin = p.window > 0 ? first + tok - p.window + 1 : 0;
+                const int free1 = max(p.causal ? min(first + 1, kv) : kv, 0) / kBlk;
+                const int free0 = p.window > 0 ? (max(first + p.tq - p.window, 0) + kBlk - 1) / kBlk : 0;
+                const int step = two ? 1 : 2;
+                for (int kb = k0 + (two ? 0 : st); kb < k1; kb += step, ++blocks) {
+                    const bool ok = __all_sync(~0u, ca_wait(s_full(st), s_phase, abort_flag, p.err));
+                    s_phase ^= 1u;
+                    tc_fence_after();
+                    // keys past the end of the cache: their V rows (the rest of a page) may hold anything
+                    auto clear_rest = [&] {
+                        if (kb * kBlk + kBlk <= kv) return;
+                        if (!two || st == 0) {
+                            const uint32_t vp = ring + 2u * (kb - k0) + 1u;
+                            ca_wait(full(vp % L::NS), (vp / L::NS) & 1u, abort_flag, p.err);
+                            const int keep = kv - kb * kBlk;
+                            uint8_t* v = smem + L::RING_OFF + (vp % L::NS) * L::TILE;
+                            for (int i = row; i < (kBlk - keep) * (D / 8); i += 128) {
+                                const int r = keep + i / (D / 8), c = i % (D / 8);
+                                *reinterpret_cast<uint4*>(v + (c / 8) * L::SUB + r * 128 + (c % 8) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                        if (two) meet();
+                    };
+                    // The two warps of a scheduler share its exponential unit: taking turns keeps the streams
+                    // half a block apart, so that one's MMAs run under the other's exponentials.
+                    auto take_turn = [&] {
+                        if (!two) return;
+                        ca_wait(my_turn, turn_phase, abort_flag, p.err);
+                        turn_phase ^= 1u;
+                        __syncwarp();
+                    };
+                    auto pass_turn = [&] {
+                        if (two && lane == 0) mbar_arrive(their_turn);
+                    };
+                    auto post = [&](uint32_t bar) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar);
+                    };
+                    if (!(warp_on && ok)) {
+                        clear_rest();
+                        take_turn();
+                        pass_turn();
+                        post(h_full(st));
+                        post(p_full(st));
+                        continue;
+                    }
                     uint32_t x[128];
-                    tc_ld32(ts, x, 0);
-                    tc_ld32(ts + 32, x, 32);
-                    tc_ld32(ts + 64, x, 64);
-                    tc_ld32(ts + 96, x, 96);
-                    tc_wait_ld32(x, 0);
-                    tc_wait_ld32(x, 32);
-                    tc_wait_ld32(x, 64);
-                    tc_wait_ld32(x, 96);
-                    const int k0 = kb * kBlk;
-                    if (k0 + kBlk > all_end || k0 < all_min) {
-                        const int je = kend - k0, jm = kmin - k0;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc_ld32(ts + 32 * c, x, 32 * c);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc_wait_ld32(x, 32 * c);
+                    if (kb >= free1 || kb < free0) {
+                        const int je = kend - kb * kBlk, jm = kmin - kb * kBlk;
 #pragma unroll
                         for (int j = 0; j < 128; ++j)
                             if (j >= je || j < jm) x[j] = 0xff800000u;
                     }
-                    float mx[4];
+                    float mx[8];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(x[c]);
+                    for (int c = 0; c < 8; ++c) mx[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[8 + c]));
 #pragma unroll
-                    for (int j = 4; j < 128; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(x[j]));
-                    const float bm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    const bool need = bm > m + lazy;
+                    for (int j = 16; j < 128; j += 16)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            mx[c] = max3(mx[c], __uint_as_float(x[j + c]), __uint_as_float(x[j + 8 + c]));
+                    const float bm = fmaxf(max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[4]), max3(mx[5], mx[6], mx[7]));
+                    const bool need = bm > m + p.lazy;
                     if (__any_sync(~0u, need)) {
                         const float mn = need ? bm : m;
                         const float a = need ? ex2((m - mn) * sl) : 1.f;
@@ -620,43 +754,57 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                             }
                         }
                     }
+                    clear_rest();
+                    take_turn();
                     const float off = m == -INFINITY ? 0.f : m * sl;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t w[64];
+                    const uint64_t sl2 = pair(sl, sl), off2 = pair(-off, -off);
+                    uint64_t sum[4] = {0, 0, 0, 0};
+                    // weights, rounded, into the place of the scores
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) {
-                        const float a = ex2(fmaf(__uint_as_float(x[2 * j]), sl, -off));
-                        const float b = ex2(fmaf(__uint_as_float(x[2 * j + 1]), sl, -off));
-                        sum[(2 * j) & 3] += a;
-                        sum[(2 * j + 1) & 3] += b;
-                        w[j] = pack2<DT>(a, b);
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int k = 64 * c + 2 * j;
+                            const uint64_t y = fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), sl2, off2);
+                            float a, b;
+                            unpair(y, a, b);
+                            a = ex2(a), b = ex2(b);
+                            sum[j & 3] = add2(sum[j & 3], pair(a, b));
+                            w[j] = pack2<DT>(a, b);
+                        }
+                        if (c == 1) pass_turn();
+                        tc_st32(ts + 32 * c, w, 0);
+                        tc_wait_st();
+                        post(c == 0 ? h_full(st) : p_full(st));
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tc_st32(ts, w, 0);
-                    tc_st32(ts + 32, w, 32);
-                    tc_wait_st();
+                    float a, b;
+                    unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+                    l += a + b;
                 }
-                // keys past the end of the cache: their V rows (the rest of a page) may hold anything
-                if (kb * kBlk + kBlk > s.r.kv && (!two || st == 0)) {
-                    const uint32_t vp = ring + 2u * (kb - s.k0) + 1u;
-                    ca_wait(full(vp % L::NS), (vp / L::NS) & 1u, abort_flag, p.err);
-                    const int keep = s.r.kv - kb * kBlk;
-                    uint8_t* v = smem + L::RING_OFF + (vp % L::NS) * L::TILE;
-                    for (int i = row; i < (kBlk - keep) * (D / 8); i += 128) {
-                        const int r = keep + i / (D / 8), c = i % (D / 8);
-                        *reinterpret_cast<uint4*>(v + (c / 8) * L::SUB + r * 128 + (c % 8) * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(st));
             }
+            const int nb = k1 - k0;
             ring += 2u * nb;
+            const int64_t orow = (int64_t)g.tok + t;
+            const int hq = g.h * p.g + row % p.g;
+            T* orow_p = static_cast<T*>(p.out) + orow * p.o_st + (int64_t)hq * p.o_sh;
+            if (nb == 0 && valid && (two || st == 0)) {   // no key is visible
+                for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(orow_p + c) = make_uint4(0u, 0u, 0u, 0u);
+                if (p.lse) p.lse[orow * p.Hq + hq] = -INFINITY;
+            }
+            const bool whole = k0 == g.lo_blk && k1 == g.hi_blk;
+            const int slot = cta * 2 + (k0 == g.lo_blk ? 1 : 0);
+            if (tid == 0 && !whole) {
+                p.rec[slot * 2] = make_int4(1, k1, g.hi_blk, g.b);
+                p.rec[slot * 2 + 1] = make_int4(g.h, g.i, 0, 0);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(seg));
+            if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
+            if (nb == 0) continue;
             if (blocks > 0) {
-                ca_wait(o_full(st), o_uses & 1u, abort_flag, p.err);
-                ++o_uses;
+                ca_wait(o_full(st), o_phase, abort_flag, p.err);
+                o_phase ^= 1u;
             }
             __syncwarp();
             tc_fence_after();
@@ -666,7 +814,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             if (!two) {
                 ml[st * 128 + row] = make_float2(mlog, l);
                 tc_fence_before();
-                wg_bar(1, 256);
+                meet();
                 tc_fence_after();
                 const float2 a = ml[row], b = ml[128 + row];
                 mlog = fmaxf(a.x, b.x);
@@ -674,34 +822,36 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 e1 = b.x == -INFINITY ? 0.f : ex2(b.x - mlog);
                 l = a.y * e0 + b.y * e1;
             }
-            const bool whole = s.whole();
             const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-            const int slot = cta * 2 + (s.k0 == s.lo_blk ? 1 : 0);
             const int prow = two ? st * 128 + row : row;
             const int c0 = two ? 0 : st * (D / 2), c1 = two ? D : c0 + D / 2;
             if (warp_on) {
                 const uint32_t t0 = tmem + lanes + kColO + (two ? D * st : 0);
-                for (int c = c0; c < c1; c += 16) {
-                    uint32_t o[16];
-                    tc_ld16(t0 + c, o);
-                    float f[16];
+                for (int c = c0; c < c1; c += 32) {
+                    uint32_t o[32], o1[32];
+                    tc_ld32(t0 + c, o, 0);
+                    const bool more = !two && nb > 1;
+                    if (more) tc_ld32(t0 + D + c, o1, 0);
+                    tc_wait_ld32(o, 0);
+                    float f[32];
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(o[j]) * e0;
-                    if (!two && nb > 1) {
-                        tc_ld16(t0 + D + c, o);
+                    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(o[j]) * e0;
+                    if (more) {
+                        tc_wait_ld32(o1, 0);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) f[j] += __uint_as_float(o[j]) * e1;
+                        for (int j = 0; j < 32; ++j) f[j] += __uint_as_float(o1[j]) * e1;
                     }
                     if (valid && whole) {
-                        uint32_t y[8];
+                        uint32_t y[16];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
-                        *reinterpret_cast<uint4*>(orow_p + c) = make_uint4(y[0], y[1], y[2], y[3]);
-                        *reinterpret_cast<uint4*>(orow_p + c + 8) = make_uint4(y[4], y[5], y[6], y[7]);
-                    } else if (valid) {
-                        float4* o4 = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * 256 + prow) * D + c);
+                        for (int j = 0; j < 16; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) o4[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                        for (int j = 0; j < 16; j += 8) st_row32(orow_p + c + 2 * j, y, j, p.out32);
+                    } else if (valid) {   // [channel / 4][row][4]: consecutive rows next to each other
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            p.part_o[((int64_t)slot * (D / 4) + c / 4 + j) * 256 + prow] =
+                                make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
                     }
                     __syncwarp();
                 }
@@ -710,12 +860,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 if (!whole) p.part_ml[slot * 256 + prow] = make_float2(mlog, l);
                 else if (p.lse) p.lse[orow * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (mlog + __log2f(l));
             }
-            if (tid == 0 && !whole) {
-                p.rec[slot * 2] = make_int4(1, s.k1, s.hi_blk, s.b);
-                p.rec[slot * 2 + 1] = make_int4(s.h, s.i, 0, 0);
-            }
             tc_fence_before();
-            if (!two) wg_bar(1, 256);
+            if (!two) meet();
         }
     }
     tc_fence_before();
@@ -726,66 +872,52 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 
 // Joins the partial outputs of the tiles that cross a cut.  The tile begun in
 // CTA c's last segment continues as the first segment of c + 1, c + 2, ...
-// until its last key block.  16 threads per row, segments in order.
+// until its last key block.  A thread per row and four channels, rows
+// fastest, segments in order.
 template <int DT, int D>
-__global__ void __launch_bounds__(kJoinRows * 16) chunk_join_kernel(const ChunkParams p, int G) {
+__global__ void __launch_bounds__(kJoinRows * D / 4) chunk_join_kernel(const ChunkParams p, int G) {
     using T = typename Elem<DT>::T;
-    constexpr int E = D / 16;
     griddep_wait();
     const int c = blockIdx.x;
     const int4 rec = p.rec[(c * 2 + 1) * 2];
     if (!rec.x) return;
     const int4 at = p.rec[(c * 2 + 1) * 2 + 1];
-    Req r = load_req(p, rec.w);
-    const int row = blockIdx.y * kJoinRows + threadIdx.x / 16, l16 = threadIdx.x % 16;
-    const int rows = min(2 * p.tq, r.qlen - at.y * 2 * p.tq) * p.g;   // tokens of the tile, all heads
-    const bool two = rows > p.tq * p.g;
-    // rows of the partials: half tiles start at 0 and 128
-    if (row >= 256) return;
-    const int half = row / 128, in_half = row % 128;
+    const Req r = load_req(p, rec.w);
+    const int row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, c4 = threadIdx.x / kJoinRows;
+    // half tiles start at rows 0 and 128
+    const int n = min(2 * p.tq, r.qlen - at.y * 2 * p.tq), half = row / 128, in_half = row % 128;
     const int tok = in_half / p.g;
-    if (tok >= p.tq || (half && !two) || (half * p.tq + tok) * p.g >= rows) return;
+    if (row >= 256 || tok >= p.tq || half * p.tq + tok >= n) return;
     // segments: c's last, then the first of the CTAs up to the one that ends the tile
     int end = c;
     for (int k1 = rec.y; k1 < rec.z && end + 1 < G;) {
-        ++end;
-        const int4 nx = p.rec[end * 4];
+        const int4 nx = p.rec[++end * 4];
         if (nx.x) k1 = nx.y;
     }
+    auto has = [&](int e) { return e == c || p.rec[e * 4].x != 0; };
     auto slot_of = [&](int e) { return e == c ? c * 2 + 1 : e * 2; };
     float m = -INFINITY;
-    auto has = [&](int e) { return e == c || p.rec[e * 4].x != 0; };
     for (int e = c; e <= end; ++e)
         if (has(e)) m = fmaxf(m, p.part_ml[slot_of(e) * 256 + row].x);
-    float l = 0.f, acc[E];
-#pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] = 0.f;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int e = c; e <= end; ++e) {
         if (!has(e)) continue;
-        const int64_t sr = (int64_t)slot_of(e) * 256 + row;
-        const float2 ml = p.part_ml[sr];
+        const float2 ml = p.part_ml[slot_of(e) * 256 + row];
+        const float4 v = p.part_o[((int64_t)slot_of(e) * (D / 4) + c4) * 256 + row];
         const float a = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
         l += ml.y * a;
-        const float4* o4 = reinterpret_cast<const float4*>(p.part_o + sr * D + l16 * E);
-#pragma unroll
-        for (int j = 0; j < E / 4; ++j) {
-            const float4 v = o4[j];
-            acc[4 * j] += v.x * a;
-            acc[4 * j + 1] += v.y * a;
-            acc[4 * j + 2] += v.z * a;
-            acc[4 * j + 3] += v.w * a;
-        }
+        acc.x += v.x * a;
+        acc.y += v.y * a;
+        acc.z += v.z * a;
+        acc.w += v.w * a;
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
     const int64_t t = (int64_t)r.q0 + at.y * 2 * p.tq + half * p.tq + tok;
     const int hq = at.x * p.g + in_half % p.g;
-    uint32_t y[E / 2];
-#pragma unroll
-    for (int j = 0; j < E / 2; ++j) y[j] = pack2<DT>(acc[2 * j] * inv, acc[2 * j + 1] * inv);
-    uint2* o = reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + l16 * E);
-#pragma unroll
-    for (int j = 0; j < E / 4; ++j) o[j] = make_uint2(y[2 * j], y[2 * j + 1]);
-    if (p.lse && l16 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4) =
+        make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+    if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
 }
 
 // ---------------------------------------------------------------------------
@@ -851,7 +983,7 @@ static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
     FADE_LAUNCH_CHECK();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(G, slices);
-    cfg.blockDim = dim3(kJoinRows * 16);
+    cfg.blockDim = dim3(kJoinRows * D / 4);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -896,7 +1028,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     p.err = reinterpret_cast<int*>(ws);
     p.rec = reinterpret_cast<int4*>(ws + 256);
     p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * 64);
-    p.part_o = reinterpret_cast<float*>(ws + 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8);
+    p.part_o = reinterpret_cast<float4*>(ws + 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8);
     p.table_stride = d->table_stride;
     p.o_st = d->o_st;
     p.o_sh = d->o_sh;
@@ -911,7 +1043,9 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     p.table_width = d->n_pages > 0 ? (int)d->table_width : 0;
     p.causal = d->causal != 0;
     p.window = d->window >= (1LL << 29) ? 0 : (int)d->window;   // as long as the longest cache: hides nothing
+    p.out32 = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_st % 16 == 0 && d->o_sh % 16 == 0;
     p.scale_log2 = (float)(d->sm_scale * 1.4426950408889634);
+    p.lazy = kLazyMax / p.scale_log2;
     CUtensorMap tq, tk, tv;
     const cuuint64_t qd[3] = {(cuuint64_t)d->D, (cuuint64_t)d->Hq, (cuuint64_t)d->T};
     const int64_t qs[2] = {d->q_sh, d->q_st};

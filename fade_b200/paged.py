@@ -274,7 +274,7 @@ _WS: dict = {}
 
 def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tensor, cu_q: Tensor, kv_lens: Tensor, *,
                     causal: bool = True, window: int | None = None, sm_scale: float | None = None,
-                    out: Tensor | None = None, return_lse: bool = False):
+                    out: Tensor | None = None, return_lse: bool = False) -> Tensor | dict:
     """Attention of a step's new tokens over their requests' paged caches.
 
     q: [T, Hq, D] fp16 or bf16, the requests' tokens one after the other
@@ -286,8 +286,9 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     ``h // (Hq // Hkv)``; sm_scale defaults to 1/sqrt(D).
 
     Returns [T, Hq, D] (zeros where no key is visible; tokens past cu_q[R] are
-    not written), with ``return_lse`` also the float32 [T, Hq] log of the sum
-    of exponentials (-inf where no key is visible).  Head_dim 64 or 128, page
+    not written); with ``return_lse`` a dict of that as "out" and the float32
+    [T, Hq] log of the sum of exponentials as "lse" (-inf where no key is
+    visible).  Head_dim 64 or 128, page
     size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
     kv_len is never used.  Workspace is cached per (device, stream); calls on
     one stream run in order, so sharing it is safe."""
@@ -341,7 +342,7 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     if ws is None or ws.numel() < need:
         ws = _WS[key] = torch.zeros(need, dtype=torch.uint8, device=dev)
     _lib.check(lib.fade_chunk_attn(ref, ws.data_ptr(), ws.numel(), st), "chunk_attention")
-    return (out, lse) if return_lse else out
+    return {"out": out, "lse": lse} if return_lse else out
 
 
 def check_device_errors(device: torch.device | str = "cuda") -> None:

@@ -487,7 +487,7 @@ def _check_attn(new, kv, hq, hkv, D, page, dt, dev, seed=0, causal=True, window=
 
     args = _attn_inputs(new, kv, hq, hkv, D, page, dt, dev, seed, layout, scale=scale)
     q, kp, vp, table = args[:4]
-    out, lse = chunk_attention(*args, causal=causal, window=window, sm_scale=sm, return_lse=True, **kw)
+    out, lse = chunk_attention(*args, causal=causal, window=window, sm_scale=sm, return_lse=True, **kw).values()
     check_device_errors(dev)
     ref, ref_lse, lim, lim_lse = _attn_ref(q, kp, vp, table, new, kv, causal, window, sm or 1 / math.sqrt(D))
     assert out.isfinite().all()
@@ -577,7 +577,7 @@ def test_chunk_attention_large_scores(cuda_device):
     pg = table[0].long()[j // 16]
     q.fill_(1.0)
     kp[pg, :, j % 16] = (j.float() / 40)[:, None, None].expand(-1, 1, 64).to(BF)
-    out, lse = chunk_attention(q, kp, vp, table, cu, kl, return_lse=True)
+    out, lse = chunk_attention(q, kp, vp, table, cu, kl, return_lse=True).values()
     ref, ref_lse, lim, lim_lse = _attn_ref(q, kp, vp, table, [3], [1500], True, None, 0.125)
     assert ((out.double() - ref).abs() <= lim).all() and ((lse.double() - ref_lse).abs() <= lim_lse).all()
 
@@ -589,7 +589,7 @@ def test_chunk_attention_repeats_bit_for_bit(cuda_device):
     other = _attn_inputs([1] * 30, [700] * 30, 8, 2, 64, 16, HF, cuda_device, 12)
     for _ in range(3):
         chunk_attention(*other)                                     # the same workspace in between
-        again, lse2 = chunk_attention(*args, return_lse=True)
+        again, lse2 = chunk_attention(*args, return_lse=True).values()
         assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
@@ -615,7 +615,7 @@ def test_chunk_attention_strides_streams_and_padding(cuda_device):
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        other, lse2 = chunk_attention(*args, return_lse=True)
+        other, lse2 = chunk_attention(*args, return_lse=True).values()
     s.synchronize()
     assert torch.equal(other, out) and torch.equal(lse2, lse)
 
