@@ -1,5 +1,7 @@
 // Page planning of a serving step and rotary positions with several axes,
 // fused with the append of K and V to a paged cache.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace fade {
@@ -52,9 +54,12 @@ __device__ __forceinline__ int row_of(const int32_t* start, int n, int x) {
     return lo;
 }
 
-// One block: lengths are scanned into shared memory (first token and first new
-// page of every request), then tokens and new pages are dealt out to threads,
-// which find their request by bisection.
+// Every block scans the lengths into its shared memory (first token and first
+// new page of every request), then takes its share of the tokens and new
+// pages, bisecting for their requests; block 0 writes what there is once.  No
+// block reads what another writes: slots in new pages come from the free list,
+// not from the table.  Latency bound (a launch, two trips to L2, a scan): 64
+// decodes 4.2 us, 2048 prompts of 131 k tokens 8.9 us (one block: 140 us).
 __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
     extern __shared__ int32_t starts[];          // [R] first token, [R] first new page
     __shared__ Sum2 warp_sums[32];
@@ -63,6 +68,7 @@ __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
     int32_t* tok0 = starts;
     int32_t* new0 = starts + R;
     const int r0 = min(R, (int)threadIdx.x * per), r1 = min(R, r0 + per);
+    const int n_free = d.n_free[0];
     Sum2 mine{0, 0};
     int bad = 0;
     for (int r = r0; r < r1; ++r) {
@@ -74,7 +80,6 @@ __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
     }
     Sum2 tot;
     const Sum2 incl = block_scan(mine, warp_sums, &tot);
-    const int n_free = d.n_free[0];
     const bool neg = __syncthreads_or(bad & 1) || n_free < 0 || n_free > d.free_cap;
     const bool full = __syncthreads_or(bad & 2);
     const int status = neg ? FADE_PLAN_LENGTHS
@@ -82,7 +87,7 @@ __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
                        : full ? FADE_PLAN_ROW_FULL
                        : tot.b > n_free ? FADE_PLAN_NO_PAGES
                                         : FADE_PLAN_OK;
-    const bool ok = status == FADE_PLAN_OK;
+    const bool ok = status == FADE_PLAN_OK, first = blockIdx.x == 0;
     Sum2 at{incl.a - mine.a, incl.b - mine.b};
     for (int r = r0; r < r1; ++r) {
         const int n = d.new_lens[r], c = d.kv_lens[r];
@@ -92,17 +97,19 @@ __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
             at.a += n;
             at.b += pages_of((int64_t)c + n, p.page_log2) - pages_of(c, p.page_log2);
         }
-        d.cu_q[r + 1] = ok ? (int)at.a : 0;
-        d.kv_out[r] = ok ? c + n : c;
+        if (first) {
+            d.cu_q[r + 1] = ok ? (int)at.a : 0;
+            d.kv_out[r] = ok ? c + n : c;
+        }
     }
-    if (threadIdx.x == 0) {
+    if (first && threadIdx.x == 0) {
         d.cu_q[0] = 0;
         d.n_free_out[0] = ok ? n_free - (int)tot.b : n_free;
         d.status[0] = status;
     }
     __syncthreads();
-    const int live = ok ? (int)tot.a : 0;
-    for (int64_t t = threadIdx.x; t < d.total; t += blockDim.x) {
+    const int live = ok ? (int)tot.a : 0, stride = gridDim.x * blockDim.x;
+    for (int64_t t = blockIdx.x * blockDim.x + threadIdx.x; t < d.total; t += stride) {
         int pos = 0;
         int64_t slot = -1;
         if (t < live) {
@@ -116,7 +123,7 @@ __global__ void __launch_bounds__(1024) plan_step_kernel(const PlanParams p) {
         d.slots[t] = slot;
     }
     const int fresh = ok ? (int)tot.b : 0;
-    for (int k = threadIdx.x; k < fresh; k += blockDim.x) {
+    for (int k = blockIdx.x * blockDim.x + threadIdx.x; k < fresh; k += stride) {
         const int r = row_of(new0, R, k);
         const int64_t j = pages_of(d.kv_lens[r], p.page_log2) + k - new0[r];
         d.block_table[r * d.table_stride + j] = d.free_pages[n_free - 1 - k];
@@ -180,65 +187,207 @@ __global__ void __launch_bounds__(1024) release_rows_kernel(const ReleaseParams 
 // Rotary positions with several axes (+ append)
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int rope_axis(const fade_rope_desc& d, int j) {
+    const int axes = (int)d.axes;
+    if (axes == 1) return 0;
     if (d.interleaved) {
-        const int a = j % (int)d.axes;
-        return a != 0 && j < d.axes * d.sections[a] ? a : 0;
+        const int a = j % axes;
+        return a != 0 && j < axes * (int)d.sections[a] ? a : 0;
     }
     int a = 0;
-    for (int64_t end = d.sections[0]; a + 1 < d.axes && j >= end; end += d.sections[a]) ++a;
+    for (int end = (int)d.sections[0]; a + 1 < axes && j >= end; end += (int)d.sections[a]) ++a;
     return a;
 }
 
-// One block per token: cos and sin of its rot/2 angles in shared memory, then
-// one thread per channel pair or copied channel.
-template <int DT>
-__global__ void __launch_bounds__(256) rope_axes_kernel(const fade_rope_desc d, int page_log2) {
+// two fp32 values per register pair, two products or sums per instruction
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 one_by_one(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// (a, b) -> (a c - b s, b c + a s): the second product rounded, the first one
+// and the sum in one operation
+template <int DT, int VEC>
+__device__ __forceinline__ void rotate_unit(typename Elem<DT>::T* a, typename Elem<DT>::T* b, const float* co, const float* si) {
+    if constexpr (VEC == 1) {
+        const float u0 = Elem<DT>::to_f(a[0]), u1 = Elem<DT>::to_f(b[0]);
+        a[0] = Elem<DT>::from_f(__fmaf_rn(u0, co[0], __fmul_rn(u1, -si[0])));
+        b[0] = Elem<DT>::from_f(__fmaf_rn(u1, co[0], __fmul_rn(u0, si[0])));
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+            const uint64_t u0 = two(Elem<DT>::to_f(a[j]), Elem<DT>::to_f(a[j + 1]));
+            const uint64_t u1 = two(Elem<DT>::to_f(b[j]), Elem<DT>::to_f(b[j + 1]));
+            const uint64_t c = two(co[j], co[j + 1]);
+            const float2 y0 = one_by_one(fma_two(u0, c, mul_two(u1, two(-si[j], -si[j + 1]))));
+            const float2 y1 = one_by_one(fma_two(u1, c, mul_two(u0, two(si[j], si[j + 1]))));
+            a[j] = Elem<DT>::from_f(y0.x), a[j + 1] = Elem<DT>::from_f(y0.y);
+            b[j] = Elem<DT>::from_f(y1.x), b[j + 1] = Elem<DT>::from_f(y1.y);
+        }
+    }
+}
+
+template <int BYTES> struct Packet;
+template <> struct Packet<16> { using T = uint4; };
+template <> struct Packet<8> { using T = uint2; };
+template <> struct Packet<4> { using T = uint32_t; };
+template <> struct Packet<2> { using T = uint16_t; };
+
+// Place of frequency j in a token's table of rot/2 cosines, then rot/2 sines:
+// packets of four of a unit apart by all units, so that neighbouring threads
+// (neighbouring units) read neighbouring 16 bytes without bank conflicts.
+template <int VEC>
+__device__ __forceinline__ int table_at(int j, int turns) {
+    return VEC < 4 ? j : (((j % VEC) / 4) * turns + j / VEC) * 4 + j % 4;
+}
+
+// A unit is VEC channels and their partners, or VEC copied channels, of up to
+// kRopeHeads heads of q, k or v of a token: its cos and sin are read and its
+// addresses made once for all of them, and their loads are in flight together.
+// A block makes the cos and sin of `tokens` tokens, then its threads share out
+// their units; the blocks of an SM hide one another's first phase.
+// HBM bound: a token's rows are read and written once.  16384 tokens of 32 + 2
+// x 8 heads of 128 bf16 channels, appended: 73 us, 5.5 TB/s of 403 MB.  With
+// one head a unit 83 us (more address arithmetic), with four 76 us; three
+// blocks per SM 78 us, five 79 us (spills); with loads under the making of the
+// next tokens' tables 87 us and more (its registers cost blocks).
+constexpr int kRopeHeads = 2;
+constexpr int kRopeBlocks = 4;   // blocks per SM
+
+template <int DT, int VEC>
+__global__ void __launch_bounds__(256, kRopeBlocks)
+    rope_axes_kernel(const __grid_constant__ fade_rope_desc d, int page_log2, int tokens) {
     using T = typename Elem<DT>::T;
-    extern __shared__ float2 cs[];
-    const int64_t t = blockIdx.x;
-    const int half = (int)d.rot / 2, D = (int)d.D;
-    for (int j = threadIdx.x; j < half; j += blockDim.x) {
-        const int64_t at = rope_axis(d, j) * d.pos_stride + t;
+    using P = typename Packet<VEC * sizeof(T)>::T;
+    extern __shared__ __align__(16) float cs[];  // [tokens][rot]
+    const int half = (int)d.rot / 2;
+    const int64_t t0 = (int64_t)blockIdx.x * tokens;
+    const int n_tok = (int)min((int64_t)tokens, d.T - t0);
+    const int turns = half / VEC, per = turns + ((int)d.D - (int)d.rot) / VEC, per_v = (int)d.D / VEC;
+    for (int a = threadIdx.x; a < n_tok * half; a += blockDim.x) {
+        const int k = a / half, j = a - k * half;
+        const int64_t at = rope_axis(d, j) * d.pos_stride + t0 + k;
         const float pos = d.positions_64 ? (float)static_cast<const int64_t*>(d.positions)[at]
                                          : (float)static_cast<const int32_t*>(d.positions)[at];
-        float s, c;
-        sincosf(__fmul_rn(pos, d.inv_freq[j]), &s, &c);
-        if (d.round_tables) s = Elem<DT>::rnd(s), c = Elem<DT>::rnd(c);
-        cs[j] = make_float2(c, d.inverse ? -s : s);
+        float s, co;
+        sincosf(__fmul_rn(pos, d.inv_freq[j]), &s, &co);
+        if (d.round_tables) s = Elem<DT>::rnd(s), co = Elem<DT>::rnd(co);
+        float* row = cs + k * 2 * half + table_at<VEC>(j, turns);
+        row[0] = co;
+        row[half] = d.inverse ? -s : s;
     }
     __syncthreads();
-    int64_t page = -1, off = 0;
-    if (d.Hkv > 0) {
-        const int64_t slot = d.slots[t];
-        if (slot >= 0 && slot < d.n_pages << page_log2) page = slot >> page_log2, off = slot & (d.page_size - 1);
-    }
-    const int per = half + D - (int)d.rot;       // pairs, then copied channels
-    auto turn = [&](const T* x, T* y, int u) {
-        if (u < half) {
-            const float a = Elem<DT>::to_f(x[u]), b = Elem<DT>::to_f(x[u + half]);
-            const float c = cs[u].x, s = cs[u].y;
-            y[u] = Elem<DT>::from_f(__fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
-            y[u + half] = Elem<DT>::from_f(__fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s)));
-        } else {
-            y[u + half] = x[u + half];
+    const int bq = ((int)d.Hq + kRopeHeads - 1) / kRopeHeads, bk = ((int)d.Hkv + kRopeHeads - 1) / kRopeHeads;
+    const int nq = bq * per, nk = bk * per, units = nq + nk + bk * per_v;
+    for (int w = threadIdx.x; w < n_tok * units; w += blockDim.x) {
+        const int k = w / units, u = w - k * units;
+        const int64_t t = t0 + k;
+        const int what = u < nq ? 0 : u < nq + nk ? 1 : 2;
+        const int i = what == 0 ? u : what == 1 ? u - nq : u - nq - nk, n = what == 2 ? per_v : per;
+        const int hb = i / n, x = i - hb * n, h0 = hb * kRopeHeads;
+        const bool turn = what != 2 && x < turns;
+        const int c = turn || what == 2 ? x * VEC : (int)d.rot + (x - turns) * VEC;   // first channel
+        const int heads = min(kRopeHeads, (int)(what == 0 ? d.Hq : d.Hkv) - h0);
+        P lo[kRopeHeads], hi[kRopeHeads];
+        {
+            const int64_t sh = what == 0 ? d.q_sh : what == 1 ? d.k_sh : d.v_sh;
+            const T* src = (what == 0   ? static_cast<const T*>(d.q) + t * d.q_st
+                            : what == 1 ? static_cast<const T*>(d.k) + t * d.k_st
+                                        : static_cast<const T*>(d.v) + t * d.v_st) + h0 * sh + c;
+#pragma unroll
+            for (int g = 0; g < kRopeHeads; ++g) {
+                if (g >= heads) continue;
+                lo[g] = *reinterpret_cast<const P*>(src + g * sh);
+                if (turn) hi[g] = *reinterpret_cast<const P*>(src + g * sh + half);
+            }
         }
-    };
-    for (int i = threadIdx.x; i < d.Hq * per; i += blockDim.x) {
-        const int64_t h = i / per;
-        turn(static_cast<const T*>(d.q) + t * d.q_st + h * d.q_sh, static_cast<T*>(d.q_out) + t * d.qo_st + h * d.qo_sh,
-             i % per);
+        int64_t sh = d.qo_sh;
+        T* dst = static_cast<T*>(d.q_out) + t * d.qo_st;
+        if (what != 0) {
+            const int64_t slot = d.slots[t];
+            if (slot < 0 || slot >= d.n_pages << page_log2) continue;   // padding
+            const int64_t page = slot >> page_log2, off = slot & (d.page_size - 1);
+            sh = what == 1 ? d.kp_sh : d.vp_sh;
+            dst = what == 1 ? static_cast<T*>(d.k_pool) + page * d.kp_sp + off * d.kp_st
+                            : static_cast<T*>(d.v_pool) + page * d.vp_sp + off * d.vp_st;
+        }
+        dst += h0 * sh + c;
+        if (turn) {
+            const float* row = cs + k * 2 * half;
+            float co[VEC], si[VEC];
+            if constexpr (VEC >= 4) {
+#pragma unroll
+                for (int j = 0; j < VEC; j += 4) {
+                    *reinterpret_cast<float4*>(co + j) = *reinterpret_cast<const float4*>(row + table_at<VEC>(c + j, turns));
+                    *reinterpret_cast<float4*>(si + j) =
+                        *reinterpret_cast<const float4*>(row + half + table_at<VEC>(c + j, turns));
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) co[j] = row[c + j], si[j] = row[half + c + j];
+            }
+#pragma unroll
+            for (int g = 0; g < kRopeHeads; ++g)
+                if (g < heads) rotate_unit<DT, VEC>(reinterpret_cast<T*>(&lo[g]), reinterpret_cast<T*>(&hi[g]), co, si);
+        }
+#pragma unroll
+        for (int g = 0; g < kRopeHeads; ++g) {
+            if (g >= heads) continue;
+            *reinterpret_cast<P*>(dst + g * sh) = lo[g];
+            if (turn) *reinterpret_cast<P*>(dst + g * sh + half) = hi[g];
+        }
     }
-    if (page < 0) return;
-    for (int i = threadIdx.x; i < d.Hkv * per; i += blockDim.x) {
-        const int64_t h = i / per;
-        turn(static_cast<const T*>(d.k) + t * d.k_st + h * d.k_sh,
-             static_cast<T*>(d.k_pool) + page * d.kp_sp + h * d.kp_sh + off * d.kp_st, i % per);
+}
+
+template <int DT, int VEC>
+static void launch_rope(const fade_rope_desc& d, int page_log2, cudaStream_t st) {
+    // up to 8 tokens a block while every block slot of the GPU still has one
+    const int64_t tokens = std::max<int64_t>(1, std::min<int64_t>(8, d.T / (148 * kRopeBlocks)));
+    const int64_t per = d.rot / 2 / VEC + (d.D - d.rot) / VEC;
+    const int64_t bq = (d.Hq + kRopeHeads - 1) / kRopeHeads, bk = (d.Hkv + kRopeHeads - 1) / kRopeHeads;
+    const int64_t units = tokens * ((bq + bk) * per + bk * (d.D / VEC));
+    const unsigned threads = units >= 256 ? 256 : (unsigned)((units + 31) / 32 * 32);
+    rope_axes_kernel<DT, VEC><<<(unsigned)((d.T + tokens - 1) / tokens), threads, (size_t)(tokens * d.rot * 4), st>>>(
+        d, page_log2, (int)tokens);
+}
+
+// The widest packet (16 bytes at most) that divides the rotated half, the
+// copied channels and the head, and to which every pointer and stride in use
+// is aligned.
+template <int DT, int VEC>
+static void launch_rope_widest(const fade_rope_desc& d, int page_log2, cudaStream_t st) {
+    using T = typename Elem<DT>::T;
+    if constexpr (VEC > 1) {
+        bool ok = (d.rot / 2) % VEC == 0 && d.D % VEC == 0 && (d.D - d.rot) % VEC == 0;
+        auto ptr = [&](const void* p) { ok = ok && reinterpret_cast<uintptr_t>(p) % (VEC * sizeof(T)) == 0; };
+        auto stride = [&](int64_t s, int64_t n) { ok = ok && (n <= 1 || s % VEC == 0); };
+        if (d.Hq > 0) {
+            ptr(d.q), ptr(d.q_out);
+            stride(d.q_st, d.T), stride(d.q_sh, d.Hq), stride(d.qo_st, d.T), stride(d.qo_sh, d.Hq);
+        }
+        if (d.Hkv > 0) {
+            ptr(d.k), ptr(d.v), ptr(d.k_pool), ptr(d.v_pool);
+            stride(d.k_st, d.T), stride(d.k_sh, d.Hkv), stride(d.v_st, d.T), stride(d.v_sh, d.Hkv);
+            stride(d.kp_sp, d.n_pages), stride(d.kp_sh, d.Hkv), stride(d.kp_st, d.page_size);
+            stride(d.vp_sp, d.n_pages), stride(d.vp_sh, d.Hkv), stride(d.vp_st, d.page_size);
+        }
+        if (!ok) return launch_rope_widest<DT, VEC / 2>(d, page_log2, st);
     }
-    for (int i = threadIdx.x; i < d.Hkv * D; i += blockDim.x) {
-        const int64_t h = i / D;
-        static_cast<T*>(d.v_pool)[page * d.vp_sp + h * d.vp_sh + off * d.vp_st + i % D] =
-            static_cast<const T*>(d.v)[t * d.v_st + h * d.v_sh + i % D];
-    }
+    launch_rope<DT, VEC>(d, page_log2, st);
 }
 
 static int log2_of(int64_t x) {
@@ -264,9 +413,14 @@ extern "C" int fade_plan_step(const fade_plan_desc* d, void* stream) {
     if (d->R > FADE_PLAN_MAX_ROWS || d->total > INT32_MAX) return FADE_ERR_UNSUPPORTED;
     PlanParams p{*d, pl};
     const size_t smem = (size_t)d->R * 8;
-    FADE_CUDA_TRY(cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       FADE_PLAN_MAX_ROWS * 8));
-    plan_step_kernel<<<1, 1024, smem, as_stream(stream)>>>(p);
+    if (smem > 40 * 1024)
+        FADE_CUDA_TRY(cudaFuncSetAttribute(plan_step_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           FADE_PLAN_MAX_ROWS * 8));
+    // threads for the longer of the scan and the tokens, a token each, up to one block per SM
+    const int64_t work = d->R > d->total ? d->R : d->total;
+    const int threads = work <= 256 ? 256 : 1024;
+    const int64_t blocks = (d->total + threads - 1) / threads;
+    plan_step_kernel<<<(unsigned)(blocks < 1 ? 1 : blocks > 148 ? 148 : blocks), threads, smem, as_stream(stream)>>>(p);
     FADE_LAUNCH_CHECK();
     return FADE_OK;
 }
@@ -281,8 +435,9 @@ extern "C" int fade_release_rows(const uint8_t* rows, int64_t R, int32_t* kv_len
     if (pl < 0 || pl > 20) return FADE_ERR_INVALID_ARG;
     if (R > FADE_PLAN_MAX_ROWS) return FADE_ERR_UNSUPPORTED;
     ReleaseParams p{rows, kv_lens, block_table, free_pages, n_free, status, table_width, table_stride, free_cap, (int)R, pl};
-    FADE_CUDA_TRY(cudaFuncSetAttribute(release_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       FADE_PLAN_MAX_ROWS * 4));
+    if (R * 4 > 40 * 1024)
+        FADE_CUDA_TRY(cudaFuncSetAttribute(release_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           FADE_PLAN_MAX_ROWS * 4));
     release_rows_kernel<<<1, 1024, (size_t)R * 4, as_stream(stream)>>>(p);
     FADE_LAUNCH_CHECK();
     return FADE_OK;
@@ -299,7 +454,7 @@ extern "C" int fade_rope_axes(const fade_rope_desc* d, void* stream) {
         sum += d->sections[a];
     }
     if (sum != d->rot / 2) return FADE_ERR_INVALID_ARG;
-    if (d->D > 4096 || d->Hq > 4096 || d->Hkv > 4096 || d->T > INT32_MAX) return FADE_ERR_UNSUPPORTED;
+    if (d->D > 1024 || d->Hq > 4096 || d->Hkv > 4096 || d->T > INT32_MAX) return FADE_ERR_UNSUPPORTED;
     if (d->T == 0 || (d->Hq == 0 && d->Hkv == 0)) return FADE_OK;
     if ((d->rot > 0 && (!d->positions || !d->inv_freq)) || (d->Hq > 0 && (!d->q || !d->q_out)))
         return FADE_ERR_INVALID_ARG;
@@ -309,11 +464,10 @@ extern "C" int fade_rope_axes(const fade_rope_desc* d, void* stream) {
         if (pl < 0 || pl > 20 || d->n_pages < 0) return FADE_ERR_INVALID_ARG;
         if (!d->k || !d->v || !d->slots || (d->n_pages > 0 && (!d->k_pool || !d->v_pool))) return FADE_ERR_INVALID_ARG;
     }
-    const size_t smem = (size_t)(d->rot / 2) * sizeof(float2);
     cudaStream_t st = as_stream(stream);
-    if (d->dtype == FADE_F16) rope_axes_kernel<FADE_F16><<<(unsigned)d->T, 256, smem, st>>>(*d, pl);
-    else if (d->dtype == FADE_BF16) rope_axes_kernel<FADE_BF16><<<(unsigned)d->T, 256, smem, st>>>(*d, pl);
-    else rope_axes_kernel<FADE_F32><<<(unsigned)d->T, 256, smem, st>>>(*d, pl);
+    if (d->dtype == FADE_F16) launch_rope_widest<FADE_F16, 8>(*d, pl, st);
+    else if (d->dtype == FADE_BF16) launch_rope_widest<FADE_BF16, 8>(*d, pl, st);
+    else launch_rope_widest<FADE_F32, 4>(*d, pl, st);
     FADE_LAUNCH_CHECK();
     return FADE_OK;
 }

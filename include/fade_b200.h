@@ -401,7 +401,7 @@ int fade_release_rows(const uint8_t* rows, int64_t R, int32_t* kv_lens, const in
  * (rounded through dtype when round_tables, as the model-side tables of 16-bit
  * models are),
  *   y[j] = x[j]*c - x[j+rot/2]*s,  y[j+rot/2] = x[j+rot/2]*c + x[j]*s
- * in fp32 (products and sums rounded separately), one rounding at the store;
+ * in fp32 (fused multiply-adds), one rounding at the store;
  * inverse = 1 negates s; channels rot..D-1 are copied.
  * q [T,Hq,D] -> q_out (may be q itself).  With Hkv > 0: k is rotated likewise
  * and, with v as it is, written to cache slot slots[t] of k_pool / v_pool
