@@ -24,7 +24,7 @@
 // constant; the sum is cut into equal parts, one per SM, wherever that falls
 // in a tile's keys (to the block of 128).  A CTA walks its contiguous range of
 // tiles; a tile that crosses a cut leaves partial outputs in the workspace,
-// joined by a second kernel.  So ragged batches, the causal triangle and few
+// joined in order by a second kernel.  So ragged batches, the causal triangle and few
 // long rows all fill the GPU alike, from lengths that only the device knows.
 //
 // Warps of a CTA: 0-3 and 4-7 softmax, 8 loads (TMA, one box per page), 9 and
@@ -33,6 +33,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <mutex>
 
@@ -45,12 +46,14 @@ constexpr int kBlk = 128;              // keys per block
 constexpr int kHalf = 128;             // rows of a half tile
 constexpr int kCaThreads = 384;
 constexpr int kCaSmemMax = 232448;     // 227 KB
-constexpr int kTileCost = 128;         // fixed cost of a tile, in keys
-constexpr int kMinShare = 256;         // least work of a CTA, in keys: one block per stream
+// Cost of a tile: a key of one half tile is 1 (a block takes about 1.2 us, at
+// HBM speed), of two half tiles 2 (2.0 us, at tensor-core speed), its start and
+// end (first loads, output) 256.
+constexpr int kTileCost = 256;
+constexpr int kMinShare = 256;         // least work of a CTA: one block per stream
 constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the maximum is moved
 constexpr uint32_t kCaPolls = 1u << 22;
 constexpr uint32_t kSegPolls = 1u << 26;
-constexpr int kJoinRows = 8;           // rows per CTA of the joining kernel
 
 struct ChunkParams {
     const int32_t* block_table;
@@ -59,10 +62,12 @@ struct ChunkParams {
     void* out;
     float* lse;
     int* err;
-    int4* rec;          // [CTA][2][2]: partial segments (continued tile, begun tile)
-    float2* part_ml;    // [CTA][2][256]: (maximum in the log2 domain, sum)
+    int4* rec;          // [CTA][2]: the tile that begins in the CTA and crosses a cut
+    float2* part_ml;    // [CTA][continued tile, begun tile][256]: (maximum in the log2 domain, sum)
     float4* part_o;     // [CTA][2][D / 4][256]
     int64_t table_stride, o_st, o_sh;
+    uint32_t tile_magic;   // division by the tokens of a tile
+    int tile_shift;
     int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32;
     float scale_log2, lazy;   // lazy: how far a score may exceed the running maximum
 };
@@ -82,23 +87,39 @@ __device__ __forceinline__ Req load_req(const ChunkParams& p, int b) {
     r.off = r.kv - r.qlen;
     return r;
 }
-// sum over i < n of clamp(a + i t, 0, L)
-__device__ __forceinline__ int64_t clamped_sum(int a, int t, int L, int n) {
-    const int n0 = a >= 0 ? 0 : (int)min((uint32_t)n, ((uint32_t)(-a) + t - 1) / t);
-    const int n1 = a >= L ? 0 : (int)min((uint32_t)n, ((uint32_t)L - (uint32_t)a + t - 1) / t);
+// x / (tokens of a tile), for 0 <= x < 2^31
+__device__ __forceinline__ uint32_t div_tile(const ChunkParams& p, uint32_t x) {
+    return __umulhi(x, p.tile_magic) >> p.tile_shift;
+}
+// sum over i < n of clamp(a + i t, 0, L), t the tokens of a tile
+__device__ __forceinline__ int64_t clamped_sum(const ChunkParams& p, int a, int L, int n) {
+    const int t = 2 * p.tq;
+    const int n0 = a >= 0 ? 0 : (int)min((uint32_t)n, div_tile(p, (uint32_t)(-a) + t - 1));
+    const int n1 = a >= L ? 0 : (int)min((uint32_t)n, div_tile(p, (uint32_t)L - (uint32_t)a + t - 1));
     const int64_t m = max(n1 - n0, 0);
     return a * m + t * (((int64_t)n0 + n1 - 1) * m / 2) + (int64_t)L * (n - max(n1, n0));
 }
-// cost of the first n tiles of a request (for one kv head)
-__device__ __forceinline__ int64_t tiles_cost(const ChunkParams& p, const Req& r, int n) {
-    const int t = 2 * p.tq;
-    int64_t c = (int64_t)kTileCost * n;
-    c += p.causal ? clamped_sum(r.off + t, t, r.kv, n) : (int64_t)r.kv * n;
-    if (p.window > 0) c -= clamped_sum(r.off - p.window + 1, t, r.kv, n);
-    return c;
-}
 __device__ __forceinline__ int tiles_of(const ChunkParams& p, const Req& r) {
-    return (r.qlen + 2 * p.tq - 1) / (2 * p.tq);
+    return (int)div_tile(p, (uint32_t)r.qlen + 2 * p.tq - 1);
+}
+// keys [lo, hi) that some row of a tile of n tokens from position pos on sees
+__device__ __forceinline__ int keys_end(const ChunkParams& p, const Req& r, int pos, int n) {
+    return p.causal ? min(max(pos + n, 0), r.kv) : r.kv;
+}
+__device__ __forceinline__ int keys_begin(const ChunkParams& p, int pos, int end) {
+    return p.window > 0 ? min(max(pos - p.window + 1, 0), end) : 0;
+}
+// cost of the first n of a request's nt tiles (for one kv head)
+__device__ __forceinline__ int64_t tiles_cost(const ChunkParams& p, const Req& r, int n, int nt) {
+    const int t = 2 * p.tq;
+    int64_t keys = p.causal ? clamped_sum(p, r.off + t, r.kv, n) : (int64_t)r.kv * n;
+    if (p.window > 0) keys -= clamped_sum(p, r.off - p.window + 1, r.kv, n);
+    int64_t c = (int64_t)kTileCost * n + 2 * keys;
+    if (n == nt && n > 0 && r.qlen - (n - 1) * t <= p.tq) {   // the last tile has one half tile only
+        const int pos = r.off + (n - 1) * t, end = keys_end(p, r, pos, r.kv - pos);
+        c -= end - keys_begin(p, pos, end);
+    }
+    return c;
 }
 
 // A tile, or the part of its key blocks that a CTA works on; handed from the
@@ -109,15 +130,38 @@ struct __align__(16) Seg {
     int kv;                    // keys of the request
     int tok, pos;              // first token (in q) and its position
     int b, h;                  // request, kv head
-    int lo_blk, hi_blk, i;     // key blocks of the whole tile, its index
-    int unused;
+    int lo_blk, hi_blk;        // key blocks of the whole tile
+    int begins, unused;        // the tile begins in this CTA
 };
 constexpr int kSegSlots = 4;
 
+// CTA c has the costs [first(c), first(c + 1)): `each`, and one more for the
+// first `rest`.
+__device__ __forceinline__ int64_t split_first(int64_t each, int rest, int c) { return each * c + min(c, rest); }
+
+// The key block that a cut at cost y of a tile falls on.
+struct Tile {
+    int lo, hi, lo_blk, hi_blk, each, cost;
+    __device__ __forceinline__ Tile(const ChunkParams& p, int pos, int n, int kv) {
+        hi = p.causal ? min(max(pos + n, 0), kv) : kv;
+        lo = keys_begin(p, pos, hi);
+        lo_blk = lo / kBlk;
+        hi_blk = hi > lo ? (hi + kBlk - 1) / kBlk : lo_blk;
+        each = n > p.tq ? 2 : 1;
+        cost = kTileCost + each * (hi - lo);
+    }
+    __device__ __forceinline__ int cut(int64_t y) const {
+        if (y <= 0) return lo_blk;
+        if (y >= cost) return hi_blk;
+        return min(max((lo + max((int)y - kTileCost, 0) / each) / kBlk, lo_blk), hi_blk);
+    }
+};
+
 struct Walk {
     Req r;
-    int b, h, i, nt;
-    int64_t pos, x0, x1;       // cost position of the tile, range of the CTA
+    int b, h, i, nt, cta, rest;
+    int64_t pos, x0, x1, each; // cost position of the tile, range of the CTA
+    int parts_from, parts_to, parts_n, parts_tok, parts_h;   // the tile that begins here and crosses x1
 
     __device__ __forceinline__ bool next(const ChunkParams& p, Seg& s) {
         while (pos < x1) {
@@ -125,22 +169,21 @@ struct Walk {
             s.n = min(t, r.qlen - t0);
             s.kv = r.kv;
             s.tok = r.q0 + t0, s.pos = r.off + t0;
-            s.b = b, s.h = h, s.i = i;
-            const int hi = p.causal ? min(max(s.pos + s.n, 0), r.kv) : r.kv;
-            const int lo = p.window > 0 ? min(max(s.pos - p.window + 1, 0), hi) : 0;
-            s.lo_blk = lo / kBlk;
-            s.hi_blk = hi > lo ? (hi + kBlk - 1) / kBlk : s.lo_blk;
-            const int cost = kTileCost + hi - lo;
-            auto cut = [&](int64_t x) {
-                const int64_t y = x - pos;
-                if (y <= 0) return s.lo_blk;
-                if (y >= cost) return s.hi_blk;
-                return min(max((lo + max((int)y - kTileCost, 0)) / kBlk, s.lo_blk), s.hi_blk);
-            };
-            s.k0 = cut(x0);
-            s.k1 = cut(x1);
-            const bool owns_start = pos >= x0;
-            pos += cost;
+            s.b = b, s.h = h;
+            const Tile tile(p, s.pos, s.n, r.kv);
+            s.lo_blk = tile.lo_blk, s.hi_blk = tile.hi_blk;
+            s.k0 = tile.cut(x0 - pos);
+            s.k1 = tile.cut(x1 - pos);
+            const bool begins = pos >= x0;
+            s.begins = begins;
+            if (begins && pos + tile.cost > x1) {   // the last tile here: which CTAs have a part of it?
+                int from = cta;
+                while (tile.cut(split_first(each, rest, from + 1) - pos) == tile.lo_blk && tile.lo_blk < tile.hi_blk) ++from;
+                int to = from;
+                while (tile.cut(split_first(each, rest, to + 1) - pos) < tile.hi_blk) ++to;
+                parts_from = from, parts_to = to, parts_n = s.n, parts_tok = s.tok, parts_h = h;
+            }
+            pos += tile.cost;
             if (++i == nt) {
                 i = 0;
                 if (++h == p.Hkv) {
@@ -152,7 +195,7 @@ struct Walk {
                     nt = tiles_of(p, r);
                 }
             }
-            if (s.k1 > s.k0 || (s.lo_blk == s.hi_blk && owns_start)) return true;
+            if (s.k1 > s.k0 || (s.lo_blk == s.hi_blk && begins)) return true;
         }
         return false;
     }
@@ -354,8 +397,6 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             mbar_init(seg_empty(x), 11);   // loads, two MMA and eight softmax warps
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        p.rec[cta * 4] = make_int4(0, 0, 0, 0);
-        p.rec[cta * 4 + 2] = make_int4(0, 0, 0, 0);
     }
     if (warp == 9) {
         tc_alloc(sb + L::MISC_OFF, 512);
@@ -369,7 +410,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         int64_t c = 0;
         for (int b = first; b < min(first + n, p.R); ++b) {
             const Req r = load_req(p, b);
-            c += tiles_cost(p, r, tiles_of(p, r));
+            const int nt = tiles_of(p, r);
+            c += tiles_cost(p, r, nt, nt);
         }
         return c;
     };
@@ -573,11 +615,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll
             for (int w = 0; w < kCaThreads / 32; ++w) W += sums[w];
             W *= p.Hkv;
-            const int n_cta = (int)min((int64_t)G, (W + kMinShare - 1) / kMinShare);
-            const int64_t each = n_cta > 0 ? W / n_cta : 0;
+            const int n_cta = W == 0 ? 0 : (int)min((int64_t)G, max((int64_t)1, W / kMinShare));
+            // (a 64-bit division costs several times a 32-bit one)
+            const int64_t each = n_cta == 0 ? 0 : W >> 32 ? W / n_cta : (int64_t)((uint32_t)W / (uint32_t)n_cta);
             const int rest = (int)(W - each * n_cta);
-            walk.x0 = cta < n_cta ? each * cta + min(cta, rest) : 0;
-            walk.x1 = cta < n_cta ? walk.x0 + each + (cta < rest ? 1 : 0) : 0;
+            walk.cta = cta, walk.each = each, walk.rest = rest, walk.parts_from = walk.parts_to = 0;
+            walk.x0 = cta < n_cta ? split_first(each, rest, cta) : 0;
+            walk.x1 = cta < n_cta ? split_first(each, rest, cta + 1) : 0;
             walk.pos = 0;
             if (cta < n_cta) {
                 // the warp's, the lane's, the request and the tile that x0 lies in
@@ -598,7 +642,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 for (;; ++walk.b) {
                     walk.r = load_req(p, walk.b);
                     walk.nt = tiles_of(p, walk.r);
-                    c = tiles_cost(p, walk.r, walk.nt);
+                    c = tiles_cost(p, walk.r, walk.nt, walk.nt);
                     if (walk.x0 < at + c * p.Hkv || walk.b + 1 >= p.R) break;
                     at += c * p.Hkv;
                 }
@@ -608,12 +652,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 walk.i = 0;
                 for (int span = walk.nt; span > 1;) {   // 32 parts of the remaining tiles
                     const int step = (span + 31) / 32, i = walk.i + lane * step;
-                    const bool below = lane * step < span && at + tiles_cost(p, walk.r, i) <= walk.x0;
+                    const bool below = lane * step < span && at + tiles_cost(p, walk.r, i, walk.nt) <= walk.x0;
                     const int k = __popc(__ballot_sync(~0u, below)) - 1;
                     span = min(step, span - k * step);
                     walk.i += k * step;
                 }
-                walk.pos = at + tiles_cost(p, walk.r, walk.i);
+                walk.pos = at + tiles_cost(p, walk.r, walk.i, walk.nt);
             }
             if (lane == 0) {
                 bool more = true;
@@ -630,6 +674,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     mbar_arrive(seg_full(seg));
                     if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
                 }
+                p.rec[cta * 2] = make_int4(walk.parts_from, walk.parts_to, walk.parts_n, walk.parts_tok);
+                p.rec[cta * 2 + 1] = make_int4(walk.parts_h, 0, 0, 0);
             }
             __syncwarp();
         }
@@ -650,6 +696,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             ca_wait(both, meetings & 1u, abort_flag, p.err);
             ++meetings;
             __syncwarp();
+        };
+        auto release = [&] {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(seg_empty(seg));
+            if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
         };
         while (true) {
             // the segment stays in its slot until this warp is through with it
@@ -725,8 +776,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     if (kb >= free1 || kb < free0) {
                         const int je = kend - kb * kBlk, jm = kmin - kb * kBlk;
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
-                            if (j >= je || j < jm) x[j] = 0xff800000u;
+                        for (int c = 0; c < 4; ++c) {   // 32 keys as a bit mask: [jm, je)
+                            const uint32_t below = je >= 32 * c + 32 ? ~0u : je > 32 * c ? (1u << (je - 32 * c)) - 1u : 0u;
+                            const uint32_t from = jm <= 32 * c ? ~0u : jm < 32 * c + 32 ? ~0u << (jm - 32 * c) : 0u;
+                            const uint32_t keep = below & from;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (!(keep >> j & 1u)) x[32 * c + j] = 0xff800000u;
+                        }
                     }
                     float mx[8];
 #pragma unroll
@@ -793,14 +850,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 if (p.lse) p.lse[orow * p.Hq + hq] = -INFINITY;
             }
             const bool whole = k0 == g.lo_blk && k1 == g.hi_blk;
-            const int slot = cta * 2 + (k0 == g.lo_blk ? 1 : 0);
-            if (tid == 0 && !whole) {
-                p.rec[slot * 2] = make_int4(1, k1, g.hi_blk, g.b);
-                p.rec[slot * 2 + 1] = make_int4(g.h, g.i, 0, 0);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(seg_empty(seg));
-            if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
+            const int slot = cta * 2 + g.begins;
+            release();
             if (nb == 0) continue;
             if (blocks > 0) {
                 ca_wait(o_full(st), o_phase, abort_flag, p.err);
@@ -870,54 +921,46 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     if (warp == 9) tc_dealloc(tmem, 512);
 }
 
-// Joins the partial outputs of the tiles that cross a cut.  The tile begun in
-// CTA c's last segment continues as the first segment of c + 1, c + 2, ...
-// until its last key block.  A thread per row and four channels, rows
-// fastest, segments in order.
+// Joins the parts of the tiles that cross a cut, in the order of the cuts.  A
+// block per CTA of the first kernel and slice of rows; a thread per row and
+// four channels, rows fastest, so that a warp reads neighbouring rows.
+constexpr int kJoinThreads = 512;
+
 template <int DT, int D>
-__global__ void __launch_bounds__(kJoinRows * D / 4) chunk_join_kernel(const ChunkParams p, int G) {
-    using T = typename Elem<DT>::T;
+__global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+    constexpr int kRows = kJoinThreads / (D / 4);
     griddep_wait();
     const int c = blockIdx.x;
-    const int4 rec = p.rec[(c * 2 + 1) * 2];
-    if (!rec.x) return;
-    const int4 at = p.rec[(c * 2 + 1) * 2 + 1];
-    const Req r = load_req(p, rec.w);
-    const int row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, c4 = threadIdx.x / kJoinRows;
-    // half tiles start at rows 0 and 128
-    const int n = min(2 * p.tq, r.qlen - at.y * 2 * p.tq), half = row / 128, in_half = row % 128;
-    const int tok = in_half / p.g;
-    if (row >= 256 || tok >= p.tq || half * p.tq + tok >= n) return;
-    // segments: c's last, then the first of the CTAs up to the one that ends the tile
-    int end = c;
-    for (int k1 = rec.y; k1 < rec.z && end + 1 < G;) {
-        const int4 nx = p.rec[++end * 4];
-        if (nx.x) k1 = nx.y;
+    const int4 rec = p.rec[c * 2];
+    const int from = rec.x, to = rec.y;
+    if (to <= from) return;
+    const int h = p.rec[c * 2 + 1].x, c4 = threadIdx.x / kRows;
+    const int rows = rec.z * p.g;                          // half tiles at rows 0 and 128 of the parts
+    for (int q = blockIdx.y * kRows + threadIdx.x % kRows; q < rows; q += gridDim.y * kRows) {
+        const int row = q < p.tq * p.g ? q : 128 + q - p.tq * p.g;
+        auto slot = [&](int e) { return e == c ? e * 2 + 1 : e * 2; };
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int e = from; e <= to; ++e) {
+            const float2 ml = p.part_ml[slot(e) * 256 + row];
+            const float4 v = p.part_o[((int64_t)slot(e) * (D / 4) + c4) * 256 + row];
+            const float mn = fmaxf(m, ml.x);
+            const float a = m == mn ? 1.f : ex2(m - mn), b = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
+            m = mn;
+            l = l * a + ml.y * b;
+            acc.x = acc.x * a + v.x * b;
+            acc.y = acc.y * a + v.y * b;
+            acc.z = acc.z * a + v.z * b;
+            acc.w = acc.w * a + v.w * b;
+        }
+        const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+        const int64_t t = (int64_t)rec.w + q / p.g;
+        const int hq = h * p.g + q % p.g;
+        *reinterpret_cast<uint2*>(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4) =
+            make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+        if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
     }
-    auto has = [&](int e) { return e == c || p.rec[e * 4].x != 0; };
-    auto slot_of = [&](int e) { return e == c ? c * 2 + 1 : e * 2; };
-    float m = -INFINITY;
-    for (int e = c; e <= end; ++e)
-        if (has(e)) m = fmaxf(m, p.part_ml[slot_of(e) * 256 + row].x);
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int e = c; e <= end; ++e) {
-        if (!has(e)) continue;
-        const float2 ml = p.part_ml[slot_of(e) * 256 + row];
-        const float4 v = p.part_o[((int64_t)slot_of(e) * (D / 4) + c4) * 256 + row];
-        const float a = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-        l += ml.y * a;
-        acc.x += v.x * a;
-        acc.y += v.y * a;
-        acc.z += v.z * a;
-        acc.w += v.w * a;
-    }
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    const int64_t t = (int64_t)r.q0 + at.y * 2 * p.tq + half * p.tq + tok;
-    const int hq = at.x * p.g + in_half % p.g;
-    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4) =
-        make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
-    if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
 }
 
 // ---------------------------------------------------------------------------
@@ -971,26 +1014,34 @@ static int make_map(CUtensorMap* m, int dtype, const void* base, int rank, const
 }
 
 static size_t ws_bytes_for(int G, int64_t D) {
-    return 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8 + (size_t)G * 2 * 256 * D * 4;
+    return 256 + (size_t)G * 32 + (size_t)G * 2 * 256 * 8 + (size_t)G * 2 * 256 * D * 4;
 }
 
 template <int DT, int D>
 static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const ChunkParams& p, int G,
-                        int slices, cudaStream_t st) {
+                        cudaStream_t st) {
     auto k = chunk_attn_kernel<DT, D>;
-    FADE_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, CaLayout<D>::BYTES));
+    static std::atomic<uint64_t> ready{0};   // devices whose kernel has its shared memory granted
+    int dev = 0;
+    FADE_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        FADE_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, CaLayout<D>::BYTES));
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     k<<<G, kCaThreads, CaLayout<D>::BYTES, st>>>(tq, tk, tv, p);
     FADE_LAUNCH_CHECK();
+    // enough blocks for the rows that a tile can have, few enough to wait beside the first kernel's
+    const int64_t rows = std::min<int64_t>(256, (int64_t)p.T * p.g);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(G, slices);
-    cfg.blockDim = dim3(kJoinRows * D / 4);
+    cfg.gridDim = dim3(G, (unsigned)std::min<int64_t>(8, (rows * (D / 4) + kJoinThreads - 1) / kJoinThreads));
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    FADE_CUDA_TRY(cudaLaunchKernelEx(&cfg, chunk_join_kernel<DT, D>, p, G));
+    FADE_CUDA_TRY(cudaLaunchKernelEx(&cfg, chunk_join_kernel<DT, D>, p));
     return FADE_OK;
 }
 
@@ -1027,8 +1078,8 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.err = reinterpret_cast<int*>(ws);
     p.rec = reinterpret_cast<int4*>(ws + 256);
-    p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * 64);
-    p.part_o = reinterpret_cast<float4*>(ws + 256 + (size_t)G * 64 + (size_t)G * 2 * 256 * 8);
+    p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * 32);
+    p.part_o = reinterpret_cast<float4*>(ws + 256 + (size_t)G * 32 + (size_t)G * 2 * 256 * 8);
     p.table_stride = d->table_stride;
     p.o_st = d->o_st;
     p.o_sh = d->o_sh;
@@ -1038,6 +1089,12 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     p.Hkv = (int)d->Hkv;
     p.g = p.Hq / p.Hkv;
     p.tq = kHalf / p.g;
+    // floor(x / t) = floor(x m / 2^(31 + s)) for x < 2^31 with s = ceil(log2 t), m = floor(2^(31 + s) / t) + 1
+    const uint32_t tile = 2 * p.tq;
+    int up = 0;
+    while ((1u << up) < tile) ++up;
+    p.tile_magic = (uint32_t)(((uint64_t)1 << (31 + up)) / tile + 1);
+    p.tile_shift = up - 1;
     while ((1 << p.page_log2) < d->page_size) ++p.page_log2;
     p.n_pages = (int)d->n_pages;
     p.table_width = d->n_pages > 0 ? (int)d->table_width : 0;
@@ -1061,12 +1118,10 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     const cuuint32_t kbox[4] = {64, (cuuint32_t)d->page_size, 1, 1};
     if ((st = make_map(&tk, (int)d->dtype, kb, 4, kd, ks, kbox)) != FADE_OK) return st;
     if ((st = make_map(&tv, (int)d->dtype, vb, 4, kd, vs, kbox)) != FADE_OK) return st;
-    const int64_t most_rows = std::min<int64_t>(256, d->T > 256 ? 256 : d->T * p.g);
-    const int slices = (int)((d->T > p.tq ? 256 : most_rows) + kJoinRows - 1) / kJoinRows;
     cudaStream_t s = as_stream(stream);
     if (d->dtype == FADE_F16)
-        return d->D == 64 ? launch_chunk<FADE_F16, 64>(tq, tk, tv, p, G, slices, s)
-                          : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, slices, s);
-    return d->D == 64 ? launch_chunk<FADE_BF16, 64>(tq, tk, tv, p, G, slices, s)
-                      : launch_chunk<FADE_BF16, 128>(tq, tk, tv, p, G, slices, s);
+        return d->D == 64 ? launch_chunk<FADE_F16, 64>(tq, tk, tv, p, G, s)
+                          : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, s);
+    return d->D == 64 ? launch_chunk<FADE_BF16, 64>(tq, tk, tv, p, G, s)
+                      : launch_chunk<FADE_BF16, 128>(tq, tk, tv, p, G, s);
 }

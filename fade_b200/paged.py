@@ -354,7 +354,10 @@ def check_device_errors(device: torch.device | str = "cuda") -> None:
     st = _lib.bind(dev)
     ws = _WS.get((dev, st))
     if ws is not None:
-        _lib.check(_lib.load().fade_workspace_check(ws.data_ptr(), ws.numel(), st), "chunk_attention")
+        status = _lib.load().fade_workspace_check(ws.data_ptr(), ws.numel(), st)
+        if status != _lib.FADE_OK:
+            del _WS[(dev, st)]          # its counters may have stopped half way
+        _lib.check(status, "chunk_attention")
 
 
 # ---------------------------------------------------------------------------
