@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -141,6 +142,12 @@ class RopeDesc(ctypes.Structure):
     ]
 
 
+# The three descriptors of the paged step are made on every call; packing one
+# from a format takes a fraction of filling a ctypes structure.
+PACK_PLAN = struct.Struct("@6q11P")
+PACK_ROPE = struct.Struct("@7q4q5q2P" + "P2q" * 4 + "P2q" + "P3q" * 2)
+
+
 class ChunkDesc(ctypes.Structure):
     _fields_ = [
         *((n, _c_i64) for n in ("dtype", "R", "T", "Hq", "Hkv", "D", "page_size", "n_pages", "table_width",
@@ -154,6 +161,8 @@ class ChunkDesc(ctypes.Structure):
         ("block_table", _vp), ("cu_q", _vp), ("kv_lens", _vp),
     ]
 
+
+PACK_CHUNK = struct.Struct("@12qd" + "P2q" * 2 + "P" + "P3q" * 2 + "3P")
 
 # (name, restype, argtypes) for every symbol of include/fade_b200.h
 _SIGNATURES = {
@@ -211,14 +220,14 @@ _SIGNATURES = {
     "fade_decode_attn_noalloc_check": (ctypes.c_int, [_vp]),
     "fade_set_middle_kernel": (ctypes.c_int, [ctypes.c_int]),
     "fade_get_middle_kernel": (ctypes.c_int, []),
-    "fade_plan_step": (ctypes.c_int, [ctypes.POINTER(PlanDesc), _vp]),
+    "fade_plan_step": (ctypes.c_int, [_vp, _vp]),
     "fade_release_rows": (
         ctypes.c_int,
         [_vp, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _vp],
     ),
-    "fade_rope_axes": (ctypes.c_int, [ctypes.POINTER(RopeDesc), _vp]),
-    "fade_chunk_attn_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(ChunkDesc)]),
-    "fade_chunk_attn": (ctypes.c_int, [ctypes.POINTER(ChunkDesc), _vp, ctypes.c_size_t, _vp]),
+    "fade_rope_axes": (ctypes.c_int, [_vp, _vp]),
+    "fade_chunk_attn_workspace_size": (ctypes.c_size_t, [_vp]),
+    "fade_chunk_attn": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 _lib = None
@@ -296,7 +305,29 @@ def bind(device: torch.device) -> int:
     if getattr(_tls, "dev", None) != idx:
         check(lib.fade_set_device(idx), "fade_set_device")
         _tls.dev = idx
-    return torch.cuda.current_stream(idx).cuda_stream
+    return _stream(idx)
+
+
+# the current stream's handle, without the stream object where torch offers that
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+
+
+def bind_index(idx: int) -> int:
+    """``bind`` for a device index."""
+    if getattr(_tls, "dev", None) != idx:
+        check(load().fade_set_device(idx), "fade_set_device")
+        _tls.dev = idx
+    return _stream(idx)
+
+
+def same_device(*tensors: torch.Tensor) -> int:
+    """Index of the CUDA device that all tensors are on (raises as ``require_cuda``)."""
+    idx = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != idx or idx < 0:
+            require_cuda(*tensors)
+    return idx
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -46,11 +46,13 @@ constexpr int kBlk = 128;              // keys per block
 constexpr int kHalf = 128;             // rows of a half tile
 constexpr int kCaThreads = 384;
 constexpr int kCaSmemMax = 232448;     // 227 KB
-// Cost of a tile: a key of one half tile is 1 (a block takes about 1.2 us, at
-// HBM speed), of two half tiles 2 (2.0 us, at tensor-core speed), its start and
-// end (first loads, output) 256.
-constexpr int kTileCost = 256;
-constexpr int kMinShare = 256;         // least work of a CTA: one block per stream
+// Cost of a tile: a key of one half tile is kCostOne (a block takes about
+// 1.25 us: HBM, or the chain of a stream), of two half tiles kCostTwo (1.85 us),
+// its start and end (first loads, output) kTileCost (about 2 us).
+constexpr int kCostOne = 2, kCostTwo = 3;
+constexpr int kTileCost = 384;
+constexpr int kMinShare = 384;         // least work of a CTA: a block per stream, and a block of any tile
+static_assert(kMinShare >= kCostTwo * kBlk, "every cut past a tile's start must move it by a block");
 constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the maximum is moved
 constexpr uint32_t kCaPolls = 1u << 22;
 constexpr uint32_t kSegPolls = 1u << 26;
@@ -114,10 +116,10 @@ __device__ __forceinline__ int64_t tiles_cost(const ChunkParams& p, const Req& r
     const int t = 2 * p.tq;
     int64_t keys = p.causal ? clamped_sum(p, r.off + t, r.kv, n) : (int64_t)r.kv * n;
     if (p.window > 0) keys -= clamped_sum(p, r.off - p.window + 1, r.kv, n);
-    int64_t c = (int64_t)kTileCost * n + 2 * keys;
+    int64_t c = (int64_t)kTileCost * n + kCostTwo * keys;
     if (n == nt && n > 0 && r.qlen - (n - 1) * t <= p.tq) {   // the last tile has one half tile only
         const int pos = r.off + (n - 1) * t, end = keys_end(p, r, pos, r.kv - pos);
-        c -= end - keys_begin(p, pos, end);
+        c -= (kCostTwo - kCostOne) * (end - keys_begin(p, pos, end));
     }
     return c;
 }
@@ -147,7 +149,7 @@ struct Tile {
         lo = keys_begin(p, pos, hi);
         lo_blk = lo / kBlk;
         hi_blk = hi > lo ? (hi + kBlk - 1) / kBlk : lo_blk;
-        each = n > p.tq ? 2 : 1;
+        each = n > p.tq ? kCostTwo : kCostOne;
         cost = kTileCost + each * (hi - lo);
     }
     __device__ __forceinline__ int cut(int64_t y) const {

@@ -21,7 +21,6 @@ The reference keeps one dense cache per batch and has no counterpart.
 
 from __future__ import annotations
 
-import ctypes
 import math
 from dataclasses import dataclass
 
@@ -40,18 +39,21 @@ _PLAN_ERRORS = {
 }
 
 
+_I32, _I64 = torch.int32, torch.int64
+
+
 def _int32(t: Tensor, shape: tuple, what: str) -> int:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
+    if t.dtype is not _I32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _table(t: Tensor, rows: int) -> tuple[int, int, int]:
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not _I32 or len(shape) != 2 or shape[0] != rows or (shape[1] > 1 and stride[1] != 1):
         raise ValueError(f"block_table must be int32 [{rows}, pages per request] with contiguous rows, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    return t.data_ptr(), t.shape[1], t.stride(0)
+                         f"{tuple(shape)}")
+    return t.data_ptr(), shape[1], stride[0]
 
 
 @dataclass
@@ -95,7 +97,11 @@ def plan_step(new_lens: Tensor, kv_lens: Tensor, block_table: Tensor, free_pages
     Lengths and the free count are inputs only: the new ones are in the plan,
     so a repeated call plans the same step.  All or nothing: a step that does
     not fit leaves the table alone and is reported by ``StepPlan.check``."""
-    dev = _lib.require_cuda(new_lens, kv_lens, block_table, free_pages, n_free)
+    if out is None:
+        dev = _lib.same_device(new_lens, kv_lens, block_table, free_pages, n_free)
+    else:
+        dev = _lib.same_device(new_lens, kv_lens, block_table, free_pages, n_free, out.cu_q, out.kv_lens, out.positions,
+                               out.slots, out.n_free, out.status)
     R, F = new_lens.numel(), free_pages.numel()
     total = int(total)
     if page_size < 1 or page_size & (page_size - 1) or page_size > 1 << 20:
@@ -106,21 +112,22 @@ def plan_step(new_lens: Tensor, kv_lens: Tensor, block_table: Tensor, free_pages
         raise ValueError(f"at most {_lib.PLAN_MAX_ROWS} requests per step, got {R}")
     bt, width, stride = _table(block_table, R)
     if out is None:
-        out = StepPlan.empty(R, total, dev)
-    else:
-        _lib.require_cuda(new_lens, out.cu_q, out.kv_lens, out.positions, out.slots, out.n_free, out.status)
-        if out.slots.dtype != torch.int64 or out.slots.shape != (total,) or not out.slots.is_contiguous():
-            raise ValueError(f"out.slots must be a contiguous int64 tensor of shape {(total,)}")
-        if out.kv_lens.data_ptr() == kv_lens.data_ptr() and R or out.n_free.data_ptr() == n_free.data_ptr():
-            raise ValueError("out must not share kv_lens or n_free with the inputs")
-    d = _lib.PlanDesc(
-        R, total, page_size, width, stride, F,
-        _int32(new_lens, (R,), "new_lens"), _int32(kv_lens, (R,), "kv_lens"), bt,
-        _int32(free_pages, (F,), "free_pages"), _int32(n_free, (1,), "n_free"), _int32(out.cu_q, (R + 1,), "out.cu_q"),
-        _int32(out.kv_lens, (R,), "out.kv_lens"), _int32(out.positions, (total,), "out.positions"),
-        out.slots.data_ptr(), _int32(out.n_free, (1,), "out.n_free"), _int32(out.status, (1,), "out.status"))
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_plan_step(ctypes.byref(d), st), "plan_step")
+        out = StepPlan.empty(R, total, new_lens.device)
+    slots = out.slots
+    if slots.dtype is not _I64 or slots.shape != (total,) or not slots.is_contiguous():
+        raise ValueError(f"out.slots must be a contiguous int64 tensor of shape {(total,)}")
+    kv_in, n_in = _int32(kv_lens, (R,), "kv_lens"), _int32(n_free, (1,), "n_free")
+    kv_out, n_out = _int32(out.kv_lens, (R,), "out.kv_lens"), _int32(out.n_free, (1,), "out.n_free")
+    if (kv_out == kv_in and R) or n_out == n_in:
+        raise ValueError("out must not share kv_lens or n_free with the inputs")
+    d = _lib.PACK_PLAN.pack(
+        R, total, page_size, width, stride, F, _int32(new_lens, (R,), "new_lens"), kv_in, bt,
+        _int32(free_pages, (F,), "free_pages"), n_in, _int32(out.cu_q, (R + 1,), "out.cu_q"), kv_out,
+        _int32(out.positions, (total,), "out.positions"), slots.data_ptr(), n_out, _int32(out.status, (1,), "out.status"))
+    st = _lib.bind_index(dev)
+    code = _lib.load().fade_plan_step(d, st)
+    if code:
+        _lib.check(code, "plan_step")
     return out
 
 
@@ -163,30 +170,46 @@ def section_axes(sections, interleaved: bool = False) -> list[int]:
     return [a for a in range(A) for _ in range(sections[a])]
 
 
-def _heads(t: Tensor, T: int, D: int, dtype: torch.dtype, what: str) -> Tensor:
-    if t.dim() != 3 or t.shape[0] != T or t.shape[2] != D or t.dtype != dtype:
-        raise ValueError(f"{what} must be [{T}, heads, {D}] in {dtype}, got {tuple(t.shape)} in {t.dtype}")
-    return t if t.stride(2) == 1 or D == 1 or t.numel() == 0 else t.contiguous()
+def _heads(t: Tensor, T: int, D: int, dtype: torch.dtype, what: str) -> tuple:
+    """(tensor with contiguous channels, heads, token stride, head stride)"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != T or shape[2] != D or t.dtype is not dtype:
+        raise ValueError(f"{what} must be [{T}, heads, {D}] in {dtype}, got {tuple(shape)} in {t.dtype}")
+    if stride[2] != 1 and D > 1 and t.numel():
+        t = t.contiguous()
+        stride = t.stride()
+    return t, shape[1], stride[0], stride[1]
 
 
-def _rope_head(x: Tensor, positions: Tensor, inv_freq: Tensor, sections) -> tuple:
-    """(positions, rot, padded sections, pos_64, pos_stride) after the checks."""
-    sections = tuple(int(s) for s in sections)
-    A, T = len(sections), x.shape[0]
+def _rope_head(x: Tensor, T: int, D: int, positions: Tensor, inv_freq: Tensor, sections) -> tuple:
+    """(positions, rot, axes, padded sections, pos_64, pos_stride) after the checks."""
+    half = inv_freq.numel()
+    sections = (half,) if sections is None else tuple(sections)
+    A = len(sections)
     if not 1 <= A <= _lib.MAX_AXES or min(sections) < 0:
         raise ValueError(f"sections must list one to {_lib.MAX_AXES} counts, got {sections}")
-    half = inv_freq.numel()
-    if inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or sum(sections) != half or 2 * half > x.shape[2]:
+    if inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous() or sum(sections) != half or 2 * half > D:
         raise ValueError(f"inv_freq must be contiguous float32 with sum(sections) = {sum(sections)} entries, at most "
-                         f"half of head_dim {x.shape[2]}, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
+                         f"half of head_dim {D}, got {inv_freq.dtype} {tuple(inv_freq.shape)}")
     if positions.dim() == 1:
         positions = positions[None]
-    if positions.shape != (A, T) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.shape != (A, T) or (positions.dtype is not _I32 and positions.dtype is not _I64):
         raise ValueError(f"positions must be int32 or int64 [{A}, {T}], got {positions.dtype} {tuple(positions.shape)}")
-    if positions.stride(1) != 1:
+    ps, one = positions.stride()
+    if one != 1:
         positions = positions.contiguous()
-    return (positions, 2 * half, sections + (0,) * (_lib.MAX_AXES - A), positions.dtype == torch.int64,
-            positions.stride(0))
+        ps = positions.stride(0)
+    return (positions, 2 * half, A, sections + (0,) * (_lib.MAX_AXES - A), positions.dtype is _I64, ps)
+
+
+def _out_heads(out: Tensor | None, x: Tensor, T: int, H: int, D: int) -> tuple:
+    """(output, token stride, head stride)"""
+    if out is None:
+        return torch.empty((T, H, D), dtype=x.dtype, device=x.device), H * D, D
+    stride = out.stride()
+    if out.shape != (T, H, D) or out.dtype is not x.dtype or (D > 1 and stride[2] != 1):
+        raise ValueError("out must match the input's shape and dtype, with contiguous channels")
+    return out, stride[0], stride[1]
 
 
 def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, interleaved: bool = False,
@@ -201,30 +224,31 @@ def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, 
     Angles, cos and sin are fp32 and the result is rounded once;
     ``round_tables`` rounds cos and sin through x's dtype first, as the tables
     of ``MRope.compute_cos_sin`` are.  ``out`` may be x itself."""
-    dev = _lib.require_cuda(x, positions, inv_freq, out)
+    dev = _lib.same_device(x, positions, inv_freq) if out is None else _lib.same_device(x, positions, inv_freq, out)
     if x.dim() != 3:
         raise ValueError(f"expected a [tokens, heads, head_dim] tensor, got shape {tuple(x.shape)}")
     T, H, D = x.shape
-    positions, rot, sec, p64, ps = _rope_head(x, positions, inv_freq, sections or (inv_freq.numel(),))
-    axes = len(sections or (0,))
-    x = _heads(x, T, D, x.dtype, "x")
-    if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=dev)
-    elif out.shape != x.shape or out.dtype != x.dtype or (D > 1 and out.stride(2) != 1):
-        raise ValueError("out must match x's shape and dtype, with contiguous channels")
-    d = _lib.RopeDesc(_lib.dtype_code(x.dtype), T, H, 0, D, rot, axes, *sec, interleaved, inverse, round_tables, p64, ps,
-                      positions.data_ptr(), inv_freq.data_ptr(), x.data_ptr(), x.stride(0), x.stride(1),
-                      out.data_ptr(), out.stride(0), out.stride(1))
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_rope_axes(ctypes.byref(d), st), "rope_axes")
+    positions, rot, axes, sec, p64, ps = _rope_head(x, T, D, positions, inv_freq, sections)
+    x, H, x_st, x_sh = _heads(x, T, D, x.dtype, "x")
+    out, o_st, o_sh = _out_heads(out, x, T, H, D)
+    d = _lib.PACK_ROPE.pack(
+        _lib.dtype_code(x.dtype), T, H, 0, D, rot, axes, *sec, interleaved, inverse, round_tables, p64, ps,
+        positions.data_ptr(), inv_freq.data_ptr(), x.data_ptr(), x_st, x_sh, out.data_ptr(), o_st, o_sh,
+        0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    st = _lib.bind_index(dev)
+    code = _lib.load().fade_rope_axes(d, st)
+    if code:
+        _lib.check(code, "rope_axes")
     return out
 
 
 def _pool(t: Tensor, heads: int, D: int, dtype: torch.dtype, what: str) -> tuple:
-    if t.dim() != 4 or t.shape[1] != heads or t.shape[3] != D or t.dtype != dtype or t.stride(3) != 1:
+    """(shape, pointer, page stride, head stride, token stride)"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 4 or shape[1] != heads or shape[3] != D or t.dtype is not dtype or stride[3] != 1:
         raise ValueError(f"{what} must be [pages, {heads}, page size, {D}] in {dtype} with contiguous channels, got "
-                         f"{tuple(t.shape)} in {t.dtype}")
-    return t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)
+                         f"{tuple(shape)} in {t.dtype}")
+    return shape, t.data_ptr(), stride[0], stride[1], stride[2]
 
 
 def rope_append(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Tensor, sections, slots: Tensor,
@@ -237,39 +261,40 @@ def rope_append(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Te
     D], any page, head and token strides; slots: int64 [T], page * page_size +
     offset (``StepPlan.slots``).  Tokens with a slot outside the pool (padding:
     -1) are rotated but not written.  ``out`` may be q itself."""
-    dev = _lib.require_cuda(q, k, v, positions, inv_freq, slots, k_pool, v_pool, out)
+    dev = _lib.same_device(q, k, v, positions, inv_freq, slots, k_pool, v_pool, q if out is None else out)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k must be [tokens, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     T, Hq, D = q.shape
-    Hkv, dtype = k.shape[1], q.dtype
-    positions, rot, sec, p64, ps = _rope_head(q, positions, inv_freq, sections or (inv_freq.numel(),))
-    axes = len(sections or (0,))
-    q, k, v = _heads(q, T, D, dtype, "q"), _heads(k, T, D, dtype, "k"), _heads(v, T, D, dtype, "v")
-    if v.shape[1] != Hkv:
-        raise ValueError(f"k and v must have the same heads, got {Hkv} and {v.shape[1]}")
-    if slots.dtype != torch.int64 or slots.shape != (T,) or not slots.is_contiguous():
+    dtype = q.dtype
+    positions, rot, axes, sec, p64, ps = _rope_head(q, T, D, positions, inv_freq, sections)
+    q, Hq, q_st, q_sh = _heads(q, T, D, dtype, "q")
+    k, Hkv, k_st, k_sh = _heads(k, T, D, dtype, "k")
+    v, Hv, v_st, v_sh = _heads(v, T, D, dtype, "v")
+    if Hv != Hkv:
+        raise ValueError(f"k and v must have the same heads, got {Hkv} and {Hv}")
+    if slots.dtype is not _I64 or slots.shape != (T,) or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 tensor of shape {(T,)}")
-    kp, vp = _pool(k_pool, Hkv, D, dtype, "k_pool"), _pool(v_pool, Hkv, D, dtype, "v_pool")
-    n_pages, page_size = k_pool.shape[0], k_pool.shape[2]
-    if page_size & (page_size - 1) or page_size < 1 or v_pool.shape != k_pool.shape:
+    shape, *kp = _pool(k_pool, Hkv, D, dtype, "k_pool")
+    v_shape, *vp = _pool(v_pool, Hkv, D, dtype, "v_pool")
+    page_size = shape[2]
+    if page_size & (page_size - 1) or page_size < 1 or v_shape != shape:
         raise ValueError("k_pool and v_pool must have one shape and a page size that is a power of two")
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != dtype or (D > 1 and out.stride(2) != 1):
-        raise ValueError("out must match q's shape and dtype, with contiguous channels")
-    d = _lib.RopeDesc(_lib.dtype_code(dtype), T, Hq, Hkv, D, rot, axes, *sec, interleaved, 0, round_tables, p64, ps,
-                      positions.data_ptr(), inv_freq.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1),
-                      out.data_ptr(), out.stride(0), out.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                      v.data_ptr(), v.stride(0), v.stride(1), slots.data_ptr(), page_size, n_pages, *kp, *vp)
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_rope_axes(ctypes.byref(d), st), "rope_append")
+    out, o_st, o_sh = _out_heads(out, q, T, Hq, D)
+    d = _lib.PACK_ROPE.pack(
+        _lib.dtype_code(dtype), T, Hq, Hkv, D, rot, axes, *sec, interleaved, 0, round_tables, p64, ps,
+        positions.data_ptr(), inv_freq.data_ptr(), q.data_ptr(), q_st, q_sh, out.data_ptr(), o_st, o_sh,
+        k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, slots.data_ptr(), page_size, shape[0], *kp, *vp)
+    st = _lib.bind_index(dev)
+    code = _lib.load().fade_rope_axes(d, st)
+    if code:
+        _lib.check(code, "rope_append")
     return out
 
 
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-_WS: dict = {}
+_WS: dict = {}          # (device, stream, head_dim) -> (workspace, address, bytes)
 
 
 def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tensor, cu_q: Tensor, kv_lens: Tensor, *,
@@ -292,72 +317,71 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
     kv_len is never used.  Workspace is cached per (device, stream); calls on
     one stream run in order, so sharing it is safe."""
-    dev = _lib.require_cuda(q, k_pool, v_pool, block_table, cu_q, kv_lens, out)
+    dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if q.dim() != 3 or k_pool.dim() != 4:
         raise ValueError(f"q must be [tokens, heads, head_dim] and k_pool [pages, heads, page size, head_dim], got "
                          f"{tuple(q.shape)} and {tuple(k_pool.shape)}")
     T, Hq, D = q.shape
-    n_pages, Hkv, page_size = k_pool.shape[:3]
     dtype = q.dtype
-    if dtype not in (torch.float16, torch.bfloat16):
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
         raise ValueError(f"unsupported dtype {dtype}; expected float16 or bfloat16")
     if D not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {D}")
+    Hkv = k_pool.shape[1]
+    shape, *kp = _pool(k_pool, Hkv, D, dtype, "k_pool")
+    v_shape, *vp = _pool(v_pool, Hkv, D, dtype, "v_pool")
+    n_pages, _, page_size, _ = shape
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page size must be one of {PAGE_SIZES}, got {page_size}")
-    if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > 128:
+    if Hkv < 1 or Hq < 1 or Hq % Hkv or Hq > 128 * Hkv:
         raise ValueError(f"Hq={Hq} must be a multiple of Hkv={Hkv}, at most 128 times it")
-    kp, vp = _pool(k_pool, Hkv, D, dtype, "k_pool"), _pool(v_pool, Hkv, D, dtype, "v_pool")
-    if v_pool.shape != k_pool.shape:
-        raise ValueError(f"k_pool and v_pool must have one shape, got {tuple(k_pool.shape)} and {tuple(v_pool.shape)}")
+    if v_shape != shape:
+        raise ValueError(f"k_pool and v_pool must have one shape, got {tuple(shape)} and {tuple(v_shape)}")
     R = kv_lens.numel()
     bt, width, stride = _table(block_table, R)
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
-    scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
+    scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"sm_scale must be positive, got {sm_scale}")
-    if q.stride(2) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()              # rows must be 16-byte aligned for the kernel's loads
+    q_st, q_sh, one = q.stride()
+    q_ptr = q.data_ptr()
+    if one != 1 or q_st % 8 or q_sh % 8 or q_ptr % 16:   # rows must be 16-byte aligned for the kernel's loads
+        q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
-    elif out.shape != (T, Hq, D) or out.dtype != dtype or out.stride(2) != 1:
-        raise ValueError("out must match q's shape and dtype, with contiguous channels")
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    d = _lib.ChunkDesc(
-        _lib.dtype_code(dtype), R, T, Hq, Hkv, D, page_size, n_pages, width, stride, causal, window or 0, scale,
-        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-        None if lse is None else lse.data_ptr(), *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"),
-        _int32(kv_lens, (R,), "kv_lens"))
+        (q_st, q_sh, _), q_ptr = q.stride(), q.data_ptr()
+    out, o_st, o_sh = _out_heads(out, q, T, Hq, D)
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    d = _lib.PACK_CHUNK.pack(
+        _lib.FADE_BF16 if dtype is torch.bfloat16 else _lib.FADE_F16, R, T, Hq, Hkv, D, page_size, n_pages, width, stride,
+        causal, window or 0, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh, 0 if lse is None else lse.data_ptr(),
+        *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"), _int32(kv_lens, (R,), "kv_lens"))
     lib = _lib.load()
-    st = _lib.bind(dev)
-    ref = ctypes.byref(d)
-    need = lib.fade_chunk_attn_workspace_size(ref)
-    if need == 0:
-        raise ValueError(f"unsupported chunk attention sizes (R={R}, T={T}, n_pages={n_pages}, table width {width})")
-    key = (dev, st)
-    ws = _WS.get(key)
-    if ws is None or ws.numel() < need:
-        ws = _WS[key] = torch.zeros(need, dtype=torch.uint8, device=dev)
-    _lib.check(lib.fade_chunk_attn(ref, ws.data_ptr(), ws.numel(), st), "chunk_attention")
+    st = _lib.bind_index(dev)
+    ws = _WS.get((dev, st, D))
+    if ws is None:
+        need = lib.fade_chunk_attn_workspace_size(d)
+        if need == 0:
+            raise ValueError(f"unsupported chunk attention sizes (R={R}, T={T}, n_pages={n_pages}, table width {width})")
+        ws = torch.zeros(need, dtype=torch.uint8, device=q.device)
+        _WS[(dev, st, D)] = ws = (ws, ws.data_ptr(), need)
+    code = lib.fade_chunk_attn(d, ws[1], ws[2], st)
+    if code:
+        _lib.check(code, "chunk_attention")
     return {"out": out, "lse": lse} if return_lse else out
 
 
 def check_device_errors(device: torch.device | str = "cuda") -> None:
     """Raise if a bounded device wait of an earlier ``chunk_attention`` call on
     the current stream gave up (synchronises)."""
-    dev = torch.device(device)
-    if dev.index is None:
-        dev = torch.device(dev.type, torch.cuda.current_device())
-    st = _lib.bind(dev)
-    ws = _WS.get((dev, st))
-    if ws is not None:
-        status = _lib.load().fade_workspace_check(ws.data_ptr(), ws.numel(), st)
-        if status != _lib.FADE_OK:
-            del _WS[(dev, st)]          # its counters may have stopped half way
-        _lib.check(status, "chunk_attention")
+    dev = torch.device(device).index
+    dev = torch.cuda.current_device() if dev is None else dev
+    st = _lib.bind_index(dev)
+    for key, (_, ptr, need) in list(_WS.items()):
+        if key[:2] == (dev, st):
+            status = _lib.load().fade_workspace_check(ptr, need, st)
+            _lib.check(status, "chunk_attention")
 
 
 # ---------------------------------------------------------------------------

@@ -180,3 +180,11 @@ def test_mrope_tables_of_several_axes():
     cfg = SimpleNamespace(head_dim=16, rope_parameters={"rope_theta": 1e4, "mrope_section": [2, 3, 3],
                                                         "mrope_interleaved": True})
     assert extract_rope_scheme(cfg).interleaved and not MRope().interleaved
+
+
+def test_packed_descriptors_have_the_structures_layout():
+    for pack, desc in ((_lib.PACK_PLAN, _lib.PlanDesc), (_lib.PACK_ROPE, _lib.RopeDesc), (_lib.PACK_CHUNK, _lib.ChunkDesc)):
+        assert pack.size == ctypes.sizeof(desc)
+        values = [float(i) if kind is ctypes.c_double else i for i, (_, kind) in enumerate(desc._fields_, 1)]
+        d = desc.from_buffer_copy(pack.pack(*values))
+        assert [getattr(d, name) for name, _ in desc._fields_] == values
