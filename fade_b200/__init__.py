@@ -19,6 +19,11 @@ _LAZY = {
     "tiered_decode_attention": ("fade_b200.attention", "tiered_decode_attention"),
     "fused_int4_sdpa": ("fade_b200.attention", "fused_int4_sdpa"),
     "TieredDecoder": ("fade_b200.decoder", "TieredDecoder"),
+    "PagedKVCache": ("fade_b200.paged", "PagedKVCache"),
+    "chunk_attention": ("fade_b200.paged", "chunk_attention"),
+    "plan_step": ("fade_b200.paged", "plan_step"),
+    "rope_append": ("fade_b200.paged", "rope_append"),
+    "rope_axes": ("fade_b200.paged", "rope_axes"),
 }
 
 
