@@ -925,42 +925,55 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 
 // Joins the parts of the tiles that cross a cut, in the order of the cuts.  A
 // block per CTA of the first kernel and slice of rows; a thread per row and
-// four channels, rows fastest, so that a warp reads neighbouring rows.
-constexpr int kJoinThreads = 512;
+// sixteen channels (four loads a part in flight, 32 bytes stored), rows
+// fastest, so that a warp reads neighbouring rows.
+constexpr int kJoinThreads = 256;
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
-    constexpr int kRows = kJoinThreads / (D / 4);
+    constexpr int kRows = kJoinThreads / (D / 16);
     griddep_wait();
     const int c = blockIdx.x;
     const int4 rec = p.rec[c * 2];
     const int from = rec.x, to = rec.y;
     if (to <= from) return;
-    const int h = p.rec[c * 2 + 1].x, c4 = threadIdx.x / kRows;
+    const int h = p.rec[c * 2 + 1].x, c4 = threadIdx.x / kRows * 4;
     const int rows = rec.z * p.g;                          // half tiles at rows 0 and 128 of the parts
     for (int q = blockIdx.y * kRows + threadIdx.x % kRows; q < rows; q += gridDim.y * kRows) {
         const int row = q < p.tq * p.g ? q : 128 + q - p.tq * p.g;
-        auto slot = [&](int e) { return e == c ? e * 2 + 1 : e * 2; };
         float m = -INFINITY, l = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 acc[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int e = from; e <= to; ++e) {
-            const float2 ml = p.part_ml[slot(e) * 256 + row];
-            const float4 v = p.part_o[((int64_t)slot(e) * (D / 4) + c4) * 256 + row];
+            const int slot = e == c ? e * 2 + 1 : e * 2;
+            const float2 ml = p.part_ml[slot * 256 + row];
+            float4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = p.part_o[((int64_t)slot * (D / 4) + c4 + j) * 256 + row];
             const float mn = fmaxf(m, ml.x);
             const float a = m == mn ? 1.f : ex2(m - mn), b = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
             m = mn;
             l = l * a + ml.y * b;
-            acc.x = acc.x * a + v.x * b;
-            acc.y = acc.y * a + v.y * b;
-            acc.z = acc.z * a + v.z * b;
-            acc.w = acc.w * a + v.w * b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[j].x = acc[j].x * a + v[j].x * b;
+                acc[j].y = acc[j].y * a + v[j].y * b;
+                acc[j].z = acc[j].z * a + v[j].z * b;
+                acc[j].w = acc[j].w * a + v[j].w * b;
+            }
         }
         const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
         const int64_t t = (int64_t)rec.w + q / p.g;
         const int hq = h * p.g + q % p.g;
-        *reinterpret_cast<uint2*>(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4) =
-            make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+        uint32_t y[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            y[2 * j] = pack2<DT>(acc[j].x * inv, acc[j].y * inv);
+            y[2 * j + 1] = pack2<DT>(acc[j].z * inv, acc[j].w * inv);
+        }
+        st_row32(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4, y, 0, p.out32);
         if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
     }
 }
@@ -1035,7 +1048,7 @@ static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
     // enough blocks for the rows that a tile can have, few enough to wait beside the first kernel's
     const int64_t rows = std::min<int64_t>(256, (int64_t)p.T * p.g);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(G, (unsigned)std::min<int64_t>(8, (rows * (D / 4) + kJoinThreads - 1) / kJoinThreads));
+    cfg.gridDim = dim3(G, (unsigned)std::min<int64_t>(8, (rows * (D / 16) + kJoinThreads - 1) / kJoinThreads));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
