@@ -24,11 +24,28 @@
 // constant; the sum is cut into equal parts, one per SM, wherever that falls
 // in a tile's keys (to the block of 128).  A CTA walks its contiguous range of
 // tiles; a tile that crosses a cut leaves partial outputs in the workspace,
-// joined in order by a second kernel.  So ragged batches, the causal triangle and few
-// long rows all fill the GPU alike, from lengths that only the device knows.
+// joined in order by a second kernel.  So ragged batches, the causal triangle
+// and few long rows all fill the GPU alike, from lengths that only the device
+// knows.
 //
 // Warps of a CTA: 0-3 and 4-7 softmax, 8 loads (TMA, one box per page), 9 and
 // 11 MMA, 10 walks the tiles and posts the segments.
+//
+// What bounds it, bf16, 32 query and 8 kv heads of 128 channels:
+//   - 4 chunks of 2048 tokens over 8192: 844-875 us, 1.18-1.22 PFLOP/s; tensor
+//     pipe 64 % and exponential unit 64 % of the cycles, at a clock that power
+//     pulls from 1.93 to below 1.75 GHz.  A block of two half tiles takes about
+//     3300 cycles against 2048 of its MMAs and 2048 of its exponentials: the
+//     streams' turns at the exponential unit (1400 each) and the chain scores
+//     - maximum - weights - weights x V are of one length.  Without turns
+//     1026 us; half of the exponentials on the FMA pipe instead (twelve
+//     instructions a pair) 995 us against 930 without.
+//   - 16 decodes of up to 8192 tokens: 74 us, 5.3 TB/s: HBM while it streams
+//     (5 TMA stages of 32 KB), the rest is start (5 us) and join (4 us).
+//   - 4 chunks of 1021 tokens, window 1024 (fp16): 99 us, 0.69 PFLOP/s: ten
+//     blocks a tile, 2.5 us of output a tile, 10 us of joining.
+// Joining in the first kernel, by the CTA that completes a tile, took longer
+// in every case (cold instructions, registers of the softmax).
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -375,7 +392,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     auto turn = [&](int x, int w) { return b1 + 8u * (13 + 2 * kSegSlots + 4 * x + w); };   // warp w of stream x may take exponentials
 
     if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
-        if (tid == 0) atomicExch(p.err, 1);
+        if (tid == 0) {
+            atomicExch(p.err, 1);
+            p.rec[cta * 2] = make_int4(0, 0, 0, 0);
+        }
         return;
     }
     if (tid == 0) {
@@ -996,7 +1016,8 @@ static PFN_cuTensorMapEncodeTiled_v12000 ca_encode_fn() {
 
 static int check_desc(const fade_chunk_desc* d) {
     if (!d || d->R < 0 || d->T < 0 || d->Hq < 1 || d->Hkv < 1 || d->Hq % d->Hkv || d->table_width < 0 ||
-        d->n_pages < 0 || d->window < 0 || !(d->sm_scale > 0.0) || std::isinf(d->sm_scale))
+        d->n_pages < 0 || d->window < 0 || !(d->sm_scale > 0.0) ||
+        !(d->sm_scale <= 1e30))
         return FADE_ERR_INVALID_ARG;
     if (d->dtype != FADE_F16 && d->dtype != FADE_BF16) return FADE_ERR_UNSUPPORTED;
     if ((d->D != 64 && d->D != 128) || d->Hq / d->Hkv > 128) return FADE_ERR_UNSUPPORTED;
@@ -1117,7 +1138,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     p.window = d->window >= (1LL << 29) ? 0 : (int)d->window;   // as long as the longest cache: hides nothing
     p.out32 = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_st % 16 == 0 && d->o_sh % 16 == 0;
     p.scale_log2 = (float)(d->sm_scale * 1.4426950408889634);
-    p.lazy = kLazyMax / p.scale_log2;
+    p.lazy = std::min(kLazyMax / p.scale_log2, 1e30f);   // finite: the first maximum always replaces -inf
     CUtensorMap tq, tk, tv;
     const cuuint64_t qd[3] = {(cuuint64_t)d->D, (cuuint64_t)d->Hq, (cuuint64_t)d->T};
     const int64_t qs[2] = {d->q_sh, d->q_st};

@@ -142,7 +142,8 @@ struct ReleaseParams {
 };
 
 // One block, in place: every read of the lengths and of the stack's height
-// precedes the barrier after which they change.
+// precedes the barrier after which they change.  Latency bound, and run when
+// requests finish, not every step.
 __global__ void __launch_bounds__(1024) release_rows_kernel(const ReleaseParams p) {
     extern __shared__ int32_t new0[];            // [R] first page a row gives back
     __shared__ Sum2 warp_sums[32];

@@ -21,7 +21,6 @@ The reference keeps one dense cache per batch and has no counterpart.
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -315,8 +314,9 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     [T, Hq] log of the sum of exponentials as "lse" (-inf where no key is
     visible).  Head_dim 64 or 128, page
     size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
-    kv_len is never used.  Workspace is cached per (device, stream); calls on
-    one stream run in order, so sharing it is safe."""
+    kv_len is never used; a NaN or infinity in a visible token's V reaches every
+    row of its tile.  Workspace is cached per (device, stream, head_dim); calls
+    on one stream run in order, so sharing it is safe."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if q.dim() != 3 or k_pool.dim() != 4:
         raise ValueError(f"q must be [tokens, heads, head_dim] and k_pool [pages, heads, page size, head_dim], got "
@@ -342,8 +342,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError(f"sm_scale must be positive, got {sm_scale}")
+    if not 0.0 < scale <= 1e30:
+        raise ValueError(f"sm_scale must be positive and at most 1e30, got {sm_scale}")
     q_st, q_sh, one = q.stride()
     q_ptr = q.data_ptr()
     if one != 1 or q_st % 8 or q_sh % 8 or q_ptr % 16:   # rows must be 16-byte aligned for the kernel's loads
