@@ -44,6 +44,14 @@
 //     (5 TMA stages of 32 KB), the rest is start (5 us) and join (4 us).
 //   - 4 chunks of 1021 tokens, window 1024 (fp16): 99 us, 0.69 PFLOP/s: ten
 //     blocks a tile, 2.5 us of output a tile, 10 us of joining.
+// V of masked keys.  A weight of zero times a NaN or an infinity is NaN in the
+// tensor core, so a V that only some rows of a tile see would reach them all.
+// The output of a tile is checked as it is written; rows that are not finite
+// are looked at again behind the join, and those with such a V among the keys
+// their mask hides are computed anew, a warp a row, from the keys they see.
+// Keys past the end of a cache are cleared in shared memory instead: what a
+// page's rest holds is anything, and there it is the common case.
+//
 // Joining in the first kernel, by the CTA that completes a tile, took longer
 // in every case (cold instructions, registers of the softmax).
 #include <cuda.h>
@@ -74,6 +82,8 @@ constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the max
 constexpr uint32_t kCaPolls = 1u << 22;
 constexpr uint32_t kSegPolls = 1u << 26;
 
+struct Walk;
+
 struct ChunkParams {
     const int32_t* block_table;
     const int32_t* cu_q;
@@ -81,10 +91,12 @@ struct ChunkParams {
     void* out;
     float* lse;
     int* err;
-    int4* rec;          // [CTA][2]: the tile that begins in the CTA and crosses a cut
+    int4* rec;          // [CTA][2]: the tile that begins in the CTA and crosses a cut; rows to look at again
+    Walk* walks;        // [CTA]: the walk of its tiles, where rows are to be looked at again
     float2* part_ml;    // [CTA][continued tile, begun tile][256]: (maximum in the log2 domain, sum)
     float4* part_o;     // [CTA][2][D / 4][256]
-    int64_t table_stride, o_st, o_sh;
+    const void *q, *k_pool, *v_pool;
+    int64_t table_stride, o_st, o_sh, q_st, q_sh, kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
     uint32_t tile_magic;   // division by the tokens of a tile
     int tile_shift;
     int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32;
@@ -180,7 +192,7 @@ struct Walk {
     Req r;
     int b, h, i, nt, cta, rest;
     int64_t pos, x0, x1, each; // cost position of the tile, range of the CTA
-    int parts_from, parts_to, parts_n, parts_tok, parts_h;   // the tile that begins here and crosses x1
+    int parts_from, parts_to, parts_n, parts_tok, parts_h, parts_b;   // the tile that begins here and crosses x1
 
     __device__ __forceinline__ bool next(const ChunkParams& p, Seg& s) {
         while (pos < x1) {
@@ -200,7 +212,7 @@ struct Walk {
                 while (tile.cut(split_first(each, rest, from + 1) - pos) == tile.lo_blk && tile.lo_blk < tile.hi_blk) ++from;
                 int to = from;
                 while (tile.cut(split_first(each, rest, to + 1) - pos) < tile.hi_blk) ++to;
-                parts_from = from, parts_to = to, parts_n = s.n, parts_tok = s.tok, parts_h = h;
+                parts_from = from, parts_to = to, parts_n = s.n, parts_tok = s.tok, parts_h = h, parts_b = b;
             }
             pos += tile.cost;
             if (++i == nt) {
@@ -355,10 +367,11 @@ struct CaLayout {
     static constexpr int ML_OFF = RING_OFF + NS * TILE;    // (m, l) of both streams
     static constexpr int BAR_OFF = ML_OFF + 2 * 128 * 8;
     static constexpr int N_BARS = 2 * NS + 21 + 2 * kSegSlots;
-    static constexpr int MISC_OFF = BAR_OFF + 8 * N_BARS;  // tensor-memory slot, abort flag
+    static constexpr int MISC_OFF = BAR_OFF + 8 * N_BARS;  // tensor-memory slot, abort flag, output not finite
     static constexpr int SEG_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
     static constexpr int SUM_OFF = SEG_OFF + kSegSlots * (int)sizeof(Seg);   // costs per warp
-    static constexpr int BYTES = SUM_OFF + kCaThreads / 32 * 8;
+    static constexpr int WALK_OFF = SUM_OFF + kCaThreads / 32 * 8;          // the walk at its start
+    static constexpr int BYTES = WALK_OFF + (int)sizeof(Walk);
     static_assert(BYTES <= kCaSmemMax, "chunk attention shared memory over the per-CTA limit");
 };
 constexpr int kColS = 0;      // two score tiles of 128 columns; the weights overlay the first 64 of each
@@ -376,6 +389,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     const int warp = __shfl_sync(~0u, tid / 32, 0);   // known to be the same for the whole warp
     const int cta = blockIdx.x, G = gridDim.x;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 8);
+    volatile int* dirty = reinterpret_cast<volatile int*>(smem + L::MISC_OFF + 12);
     const uint32_t bars = sb + L::BAR_OFF;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (L::NS + s); };
@@ -394,12 +408,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
         if (tid == 0) {
             atomicExch(p.err, 1);
-            p.rec[cta * 2] = make_int4(0, 0, 0, 0);
+            p.rec[cta * 2] = p.rec[cta * 2 + 1] = make_int4(0, 0, 0, 0);
         }
         return;
     }
     if (tid == 0) {
-        *abort_flag = 0;
+        *abort_flag = *dirty = 0;
         for (int s = 0; s < L::NS; ++s) {
             mbar_init(full(s), 1);
             mbar_init(empty(s), 2);
@@ -682,6 +696,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 walk.pos = at + tiles_cost(p, walk.r, walk.i, walk.nt);
             }
             if (lane == 0) {
+                *reinterpret_cast<Walk*>(smem + L::WALK_OFF) = walk;
                 bool more = true;
                 while (more) {
                     more = walk.next(p, s);
@@ -697,7 +712,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
                 }
                 p.rec[cta * 2] = make_int4(walk.parts_from, walk.parts_to, walk.parts_n, walk.parts_tok);
-                p.rec[cta * 2 + 1] = make_int4(walk.parts_h, 0, 0, 0);
+                p.rec[cta * 2 + 1] = make_int4(walk.parts_h, 0, walk.parts_b, 0);
             }
             __syncwarp();
         }
@@ -898,6 +913,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
             const int prow = two ? st * 128 + row : row;
             const int c0 = two ? 0 : st * (D / 2), c1 = two ? D : c0 + D / 2;
+            uint64_t zero = 0;          // NaN once an output is not finite
             if (warp_on) {
                 const uint32_t t0 = tmem + lanes + kColO + (two ? D * st : 0);
                 for (int c = c0; c < c1; c += 32) {
@@ -917,6 +933,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     if (valid && whole) {
                         uint32_t y[16];
 #pragma unroll
+                        for (int j = 0; j < 16; ++j) zero = fma2(pair(f[2 * j], f[2 * j + 1]), 0, zero);
+#pragma unroll
                         for (int j = 0; j < 16; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
 #pragma unroll
                         for (int j = 0; j < 16; j += 8) st_row32(orow_p + c + 2 * j, y, j, p.out32);
@@ -929,6 +947,9 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     __syncwarp();
                 }
             }
+            float z0, z1;
+            unpair(zero, z0, z1);
+            if (!(z0 + z1 == 0.f)) *dirty = 1;
             if (valid && (two || st == 0)) {
                 if (!whole) p.part_ml[slot * 256 + prow] = make_float2(mlog, l);
                 else if (p.lse) p.lse[orow * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (mlog + __log2f(l));
@@ -941,6 +962,105 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     __syncthreads();
     tc_fence_after();
     if (warp == 9) tc_dealloc(tmem, 512);
+    if (tid == 0 && *dirty) {
+        p.walks[cta] = *reinterpret_cast<Walk*>(smem + L::WALK_OFF);
+        reinterpret_cast<int*>(p.rec + cta * 2 + 1)[1] = 1;
+    }
+}
+
+// A warp looks again at the output of one row, which sees the keys [kmin, kend)
+// of the [lo, hi) that its tile went through.  If it is not finite and a V of
+// the tile's other keys is not, it is computed anew.
+template <int DT, int D>
+__device__ __noinline__ void mend_row(const ChunkParams& p, int b, int h, int hq, int64_t t, int kmin, int kend, int lo,
+                                      int hi) {
+    using T = typename Elem<DT>::T;
+    constexpr int N = D / 32;                              // channels of a lane
+    const int lane = threadIdx.x % 32;
+    T* out = static_cast<T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + lane * N;
+    auto finite = [](const T* x) {
+        bool ok = true;
+#pragma unroll
+        for (int c = 0; c < N; ++c) ok &= isfinite(Elem<DT>::to_f(x[c]));
+        return ok;
+    };
+    if (__all_sync(~0u, finite(out))) return;
+    const int32_t* row = p.block_table + b * p.table_stride;
+    const T* kp = static_cast<const T*>(p.k_pool) + h * p.kp_sh + lane * N;
+    const T* vp = static_cast<const T*>(p.v_pool) + h * p.vp_sh + lane * N;
+    const int in_page = (1 << p.page_log2) - 1;
+    bool bad = false;
+    for (int j = lo; j < hi; ++j) {
+        if (j >= kmin && j < kend) {
+            j = kend - 1;
+            continue;
+        }
+        const int64_t id = row[j >> p.page_log2];
+        if (id >= 0 && id < p.n_pages) bad |= !finite(vp + id * p.vp_sp + (j & in_page) * p.vp_st);
+    }
+    if (!__any_sync(~0u, bad)) return;
+    const T* qp = static_cast<const T*>(p.q) + t * p.q_st + (int64_t)hq * p.q_sh + lane * N;
+    float m = -INFINITY, l = 0.f, acc[N], q[N];
+#pragma unroll
+    for (int c = 0; c < N; ++c) acc[c] = 0.f, q[c] = Elem<DT>::to_f(qp[c]);
+    for (int j = kmin; j < kend; ++j) {
+        const int64_t id = row[j >> p.page_log2];
+        const bool in = id >= 0 && id < p.n_pages;         // beyond the pool: zeros
+        float s = 0.f, v[N];
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            s += in ? q[c] * Elem<DT>::to_f(kp[id * p.kp_sp + (j & in_page) * p.kp_st + c]) : 0.f;
+            v[c] = in ? Elem<DT>::to_f(vp[id * p.vp_sp + (j & in_page) * p.vp_st + c]) : 0.f;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        s *= p.scale_log2;
+        const float mn = fmaxf(m, s), off = mn == -INFINITY ? 0.f : mn;
+        const float a = ex2(m - off), w = ex2(s - off);
+        m = mn;
+        l = l * a + w;
+#pragma unroll
+        for (int c = 0; c < N; ++c) acc[c] = acc[c] * a + w * v[c];
+    }
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+#pragma unroll
+    for (int c = 0; c < N; ++c) out[c] = Elem<DT>::from_f(acc[c] * inv);
+}
+// The rows q0, q0 + step, ... below end of a tile
+template <int DT, int D>
+__device__ __noinline__ void mend_tile(const ChunkParams& p, const Seg& s, int q0, int step, int end) {
+    for (int q = q0; q < end; q += step) {
+        const int pos = s.pos + q / p.g;
+        const int kend = p.causal ? min(max(pos + 1, 0), s.kv) : s.kv;
+        const int kmin = p.window > 0 ? min(max(pos - p.window + 1, 0), kend) : 0;
+        mend_row<DT, D>(p, s.b, s.h, s.h * p.g + q % p.g, (int64_t)s.tok + q / p.g, kmin, kend, s.lo_blk * kBlk,
+                        min(s.hi_blk * kBlk, s.kv));
+    }
+}
+
+// The tiles that CTA c wrote itself, their rows over the blocks of a column of the grid
+template <int DT, int D>
+__device__ __noinline__ void mend_written(const ChunkParams& p, int c) {
+    const int warps = blockDim.x / 32;
+    Walk walk = p.walks[c];
+    Seg s;
+    while (walk.next(p, s))
+        if (s.k0 == s.lo_blk && s.k1 == s.hi_blk && s.k1 > s.k0)
+            mend_tile<DT, D>(p, s, blockIdx.y * warps + threadIdx.x / 32, gridDim.y * warps, s.n * p.g);
+}
+// The rows of the tile begun in CTA c that this block has joined, `rows` at a time
+template <int DT, int D>
+__device__ __noinline__ void mend_joined(const ChunkParams& p, int c, int rows) {
+    const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
+    const Req r = load_req(p, more.z);
+    Seg s;
+    s.n = rec.z, s.tok = rec.w, s.b = more.z, s.h = more.x, s.kv = r.kv;
+    s.pos = r.off + s.tok - r.q0;
+    const Tile tile(p, s.pos, s.n, r.kv);
+    s.lo_blk = tile.lo_blk, s.hi_blk = tile.hi_blk;
+    const int end = s.n * p.g;
+    for (int q = blockIdx.y * rows; q < end; q += gridDim.y * rows)
+        mend_tile<DT, D>(p, s, q + threadIdx.x / 32, blockDim.x / 32, min(q + rows, end));
 }
 
 // Joins the parts of the tiles that cross a cut, in the order of the cuts.  A
@@ -950,14 +1070,16 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 constexpr int kJoinThreads = 256;
 
 template <int DT, int D>
-__global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int kRows = kJoinThreads / (D / 16);
     griddep_wait();
     const int c = blockIdx.x;
-    const int4 rec = p.rec[c * 2];
+    const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
     const int from = rec.x, to = rec.y;
+    if (more.y) mend_written<DT, D>(p, c);
     if (to <= from) return;
-    const int h = p.rec[c * 2 + 1].x, c4 = threadIdx.x / kRows * 4;
+    const int h = more.x, c4 = threadIdx.x / kRows * 4;
+    bool bad = false;
     const int rows = rec.z * p.g;                          // half tiles at rows 0 and 128 of the parts
     for (int q = blockIdx.y * kRows + threadIdx.x % kRows; q < rows; q += gridDim.y * kRows) {
         const int row = q < p.tq * p.g ? q : 128 + q - p.tq * p.g;
@@ -988,14 +1110,18 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_join_kernel(const __grid_c
         const int64_t t = (int64_t)rec.w + q / p.g;
         const int hq = h * p.g + q % p.g;
         uint32_t y[8];
+        float zero = 0.f;                                  // NaN if an output is not finite
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             y[2 * j] = pack2<DT>(acc[j].x * inv, acc[j].y * inv);
             y[2 * j + 1] = pack2<DT>(acc[j].z * inv, acc[j].w * inv);
+            zero = fmaf(acc[j].x, 0.f, fmaf(acc[j].y, 0.f, fmaf(acc[j].z, 0.f, fmaf(acc[j].w, 0.f, zero))));
         }
+        bad |= !(zero == 0.f);
         st_row32(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4, y, 0, p.out32);
         if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
     }
+    if (__syncthreads_or(bad)) mend_joined<DT, D>(p, c, kRows);
 }
 
 // ---------------------------------------------------------------------------
@@ -1049,8 +1175,10 @@ static int make_map(CUtensorMap* m, int dtype, const void* base, int rank, const
     return r == CUDA_SUCCESS ? FADE_OK : FADE_ERR_ALIGN;
 }
 
+constexpr int kWalkBytes = 128;   // of a CTA in the workspace
+static_assert(sizeof(Walk) <= kWalkBytes);
 static size_t ws_bytes_for(int G, int64_t D) {
-    return 256 + (size_t)G * 32 + (size_t)G * 2 * 256 * 8 + (size_t)G * 2 * 256 * D * 4;
+    return 256 + (size_t)G * (32 + kWalkBytes) + (size_t)G * 2 * 256 * 8 + (size_t)G * 2 * 256 * D * 4;
 }
 
 template <int DT, int D>
@@ -1114,11 +1242,23 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.err = reinterpret_cast<int*>(ws);
     p.rec = reinterpret_cast<int4*>(ws + 256);
-    p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * 32);
-    p.part_o = reinterpret_cast<float4*>(ws + 256 + (size_t)G * 32 + (size_t)G * 2 * 256 * 8);
+    p.walks = reinterpret_cast<Walk*>(ws + 256 + (size_t)G * 32);
+    p.part_ml = reinterpret_cast<float2*>(ws + 256 + (size_t)G * (32 + kWalkBytes));
+    p.part_o = reinterpret_cast<float4*>(ws + 256 + (size_t)G * (32 + kWalkBytes) + (size_t)G * 2 * 256 * 8);
     p.table_stride = d->table_stride;
     p.o_st = d->o_st;
     p.o_sh = d->o_sh;
+    p.q = d->q;
+    p.q_st = d->q_st;
+    p.q_sh = d->q_sh;
+    p.k_pool = d->k_pool;
+    p.kp_sp = d->kp_sp;
+    p.kp_sh = d->kp_sh;
+    p.kp_st = d->kp_st;
+    p.v_pool = d->v_pool;
+    p.vp_sp = d->vp_sp;
+    p.vp_sh = d->vp_sh;
+    p.vp_st = d->vp_st;
     p.R = (int)d->R;
     p.T = (int)d->T;
     p.Hq = (int)d->Hq;

@@ -755,3 +755,43 @@ def test_cache_steps_and_release(cuda_device):
     held = [cache.block_table[r, :-(-lens[r] // page)].tolist() for r in range(R)]
     pages = sum(held, []) + cache.free_pages[:cache.n_free.item()].tolist()
     assert sorted(pages) == list(range(40))                        # every page in one place
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("new,kv,hq,hkv,D,page,dt,causal,window,where", [
+    ([5], [3000], 8, 1, 128, 64, BF, True, None, {0: [2999, 2997]}),          # later drafts, a tile over many SMs
+    ([5] * 16, [900 + 37 * r for r in range(16)], 32, 8, 128, 32, HF, True, None, {3: [1010], 9: [1231, 1232]}),
+    ([300], [700], 8, 2, 64, 16, HF, True, None, {0: [450, 640, 699]}),       # inside the chunk
+    ([129], [129], 4, 4, 64, 32, BF, True, None, {0: [0, 128]}),              # the first key reaches every row
+    ([200, 1], [1200, 700], 16, 4, 128, 16, BF, True, 64, {0: [990, 1100], 1: [630, 636]}),
+    ([1, 1, 1], [1000, 60, 5], 14, 2, 64, 64, HF, True, 129, {0: [800, 870]}),      # before every row's window
+    ([130], [100], 8, 2, 64, 16, HF, True, None, {0: [99, 40]}),              # rows without keys beside it
+    ([40], [500], 8, 2, 128, 128, BF, False, 300, {0: [170, 210]}),
+    ([1021], [4000], 8, 2, 128, 128, HF, True, 1024, {0: [2100, 3500]}),
+])
+def test_chunk_attention_masked_values(cuda_device, new, kv, hq, hkv, D, page, dt, causal, window, where, bad):
+    """A NaN or an infinity in V reaches the rows that see its key, in its channel, and nothing else."""
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    q, kp, vp, table, cu, kl = _attn_inputs(new, kv, hq, hkv, D, page, dt, cuda_device, 21)
+    clean = vp.clone()
+    ref, ref_lse, lim, lim_lse = _attn_ref(q, kp, clean, table, new, kv, causal, window, D ** -0.5)
+    hit = torch.zeros_like(ref, dtype=torch.bool)
+    t0 = 0
+    for r, n in enumerate(new):
+        for j in where.get(r, ()):
+            chan = (7 * j) % D
+            vp[int(table[r, j // page]), :, j % page, chan] = bad
+            p = kv[r] - n + torch.arange(n, device=cuda_device)
+            sees = ((p >= j) if causal else p >= -n) & ((p - window < j) if window else p >= -n)
+            hit[t0:t0 + n, :, chan] |= sees[:, None]
+        t0 += n
+    out, lse = chunk_attention(q, kp, vp, table, cu, kl, causal=causal, window=window, return_lse=True).values()
+    check_device_errors(cuda_device)
+    assert not out[hit].isfinite().any()
+    assert out[~hit].isfinite().all()
+    assert ((out.double() - ref).abs() <= lim)[~hit].all()
+    some = ~ref_lse.isinf()
+    assert torch.equal(~lse.isinf(), some) and ((lse.double() - ref_lse).abs() <= lim_lse)[some].all()
+    again = chunk_attention(q, kp, clean, table, cu, kl, causal=causal, window=window)   # nothing stays behind
+    assert again.isfinite().all() and ((again.double() - ref).abs() <= lim).all()
