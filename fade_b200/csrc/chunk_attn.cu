@@ -40,9 +40,9 @@
 //     - maximum - weights - weights x V are of one length.  Without turns
 //     1026 us; half of the exponentials on the FMA pipe instead (twelve
 //     instructions a pair) 995 us against 930 without.
-//   - 16 decodes of up to 8192 tokens: 74 us, 5.3 TB/s: HBM while it streams
+//   - 16 decodes of up to 8192 tokens: 76 us, 5.2 TB/s: HBM while it streams
 //     (5 TMA stages of 32 KB), the rest is start (5 us) and join (4 us).
-//   - 4 chunks of 1021 tokens, window 1024 (fp16): 99 us, 0.69 PFLOP/s: ten
+//   - 4 chunks of 1021 tokens, window 1024 (fp16): 101 us, 0.67 PFLOP/s: ten
 //     blocks a tile, 2.5 us of output a tile, 10 us of joining.
 // V of masked keys.  A weight of zero times a NaN or an infinity is NaN in the
 // tensor core, so a V that only some rows of a tile see would reach them all.
@@ -972,7 +972,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 // of the [lo, hi) that its tile went through.  If it is not finite and a V of
 // the tile's other keys is not, it is computed anew.
 template <int DT, int D>
-__device__ __noinline__ void mend_row(const ChunkParams& p, int b, int h, int hq, int64_t t, int kmin, int kend, int lo,
+__device__ __forceinline__ void mend_row(const ChunkParams& p, int b, int h, int hq, int64_t t, int kmin, int kend, int lo,
                                       int hi) {
     using T = typename Elem<DT>::T;
     constexpr int N = D / 32;                              // channels of a lane
@@ -1028,7 +1028,7 @@ __device__ __noinline__ void mend_row(const ChunkParams& p, int b, int h, int hq
 }
 // The rows q0, q0 + step, ... below end of a tile
 template <int DT, int D>
-__device__ __noinline__ void mend_tile(const ChunkParams& p, const Seg& s, int q0, int step, int end) {
+__device__ __forceinline__ void mend_tile(const ChunkParams& p, const Seg& s, int q0, int step, int end) {
     for (int q = q0; q < end; q += step) {
         const int pos = s.pos + q / p.g;
         const int kend = p.causal ? min(max(pos + 1, 0), s.kv) : s.kv;
@@ -1038,35 +1038,38 @@ __device__ __noinline__ void mend_tile(const ChunkParams& p, const Seg& s, int q
     }
 }
 
-// The tiles that CTA c wrote itself, their rows over the blocks of a column of the grid
+// The rows of the tile begun in CTA c that this block has joined, `rows` at a time,
+// and the tiles that the CTA wrote itself, their rows over the blocks of a column
+// of the grid
 template <int DT, int D>
-__device__ __noinline__ void mend_written(const ChunkParams& p, int c) {
-    const int warps = blockDim.x / 32;
-    Walk walk = p.walks[c];
+__device__ __forceinline__ void mend(const ChunkParams& p, int c, int rows) {
+    const int warps = blockDim.x / 32, warp = threadIdx.x / 32;
+    const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
     Seg s;
+    if (rec.y > rec.x) {
+        const Req r = load_req(p, more.z);
+        s.n = rec.z, s.tok = rec.w, s.b = more.z, s.h = more.x, s.kv = r.kv;
+        s.pos = r.off + s.tok - r.q0;
+        const Tile tile(p, s.pos, s.n, r.kv);
+        s.lo_blk = tile.lo_blk, s.hi_blk = tile.hi_blk;
+        const int end = s.n * p.g;
+        for (int q = blockIdx.y * rows; q < end; q += gridDim.y * rows)
+            mend_tile<DT, D>(p, s, q + warp, warps, min(q + rows, end));
+    }
+    if (!more.y) return;
+    Walk walk = p.walks[c];
     while (walk.next(p, s))
         if (s.k0 == s.lo_blk && s.k1 == s.hi_blk && s.k1 > s.k0)
-            mend_tile<DT, D>(p, s, blockIdx.y * warps + threadIdx.x / 32, gridDim.y * warps, s.n * p.g);
-}
-// The rows of the tile begun in CTA c that this block has joined, `rows` at a time
-template <int DT, int D>
-__device__ __noinline__ void mend_joined(const ChunkParams& p, int c, int rows) {
-    const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
-    const Req r = load_req(p, more.z);
-    Seg s;
-    s.n = rec.z, s.tok = rec.w, s.b = more.z, s.h = more.x, s.kv = r.kv;
-    s.pos = r.off + s.tok - r.q0;
-    const Tile tile(p, s.pos, s.n, r.kv);
-    s.lo_blk = tile.lo_blk, s.hi_blk = tile.hi_blk;
-    const int end = s.n * p.g;
-    for (int q = blockIdx.y * rows; q < end; q += gridDim.y * rows)
-        mend_tile<DT, D>(p, s, q + threadIdx.x / 32, blockDim.x / 32, min(q + rows, end));
+            mend_tile<DT, D>(p, s, blockIdx.y * warps + warp, gridDim.y * warps, s.n * p.g);
 }
 
 // Joins the parts of the tiles that cross a cut, in the order of the cuts.  A
 // block per CTA of the first kernel and slice of rows; a thread per row and
 // sixteen channels (four loads a part in flight, 32 bytes stored), rows
 // fastest, so that a warp reads neighbouring rows.
+// Mending is inlined and capped at three blocks per SM: as calls it needs a
+// stack, and 16 decodes take 76.3 us against 75.6 (74.0 without it); without
+// the cap 77.3.
 constexpr int kJoinThreads = 256;
 
 template <int DT, int D>
@@ -1076,11 +1079,10 @@ __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __gri
     const int c = blockIdx.x;
     const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
     const int from = rec.x, to = rec.y;
-    if (more.y) mend_written<DT, D>(p, c);
-    if (to <= from) return;
+    if (to <= from && !more.y) return;
     const int h = more.x, c4 = threadIdx.x / kRows * 4;
     bool bad = false;
-    const int rows = rec.z * p.g;                          // half tiles at rows 0 and 128 of the parts
+    const int rows = to > from ? rec.z * p.g : 0;          // half tiles at rows 0 and 128 of the parts
     for (int q = blockIdx.y * kRows + threadIdx.x % kRows; q < rows; q += gridDim.y * kRows) {
         const int row = q < p.tq * p.g ? q : 128 + q - p.tq * p.g;
         float m = -INFINITY, l = 0.f;
@@ -1121,7 +1123,7 @@ __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __gri
         st_row32(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4, y, 0, p.out32);
         if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));
     }
-    if (__syncthreads_or(bad)) mend_joined<DT, D>(p, c, kRows);
+    if (__syncthreads_or(bad || more.y)) mend<DT, D>(p, c, kRows);
 }
 
 // ---------------------------------------------------------------------------
@@ -1224,7 +1226,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     if (bad != FADE_OK) return bad;
     if (d->T == 0 || d->R == 0) return FADE_OK;
     if (!d->q || !d->out || !d->cu_q || !d->kv_lens || (d->table_width > 0 && !d->block_table) ||
-        (d->n_pages > 0 && (!d->k_pool || !d->v_pool)))
+        (d->n_pages > 0 && (!d->k_pool || !d->v_pool)) || d->out == d->q)
         return FADE_ERR_INVALID_ARG;
     const int64_t strides[] = {d->q_st, d->q_sh, d->o_st, d->o_sh, d->kp_sp, d->kp_sh, d->kp_st, d->vp_sp, d->vp_sh, d->vp_st};
     for (int64_t s : strides)

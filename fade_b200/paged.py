@@ -314,8 +314,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     [T, Hq] log of the sum of exponentials as "lse" (-inf where no key is
     visible).  Head_dim 64 or 128, page
     size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
-    kv_len is never used; a NaN or infinity in a visible token's V reaches every
-    row of its tile.  Workspace is cached per (device, stream, head_dim); calls
+    kv_len is never used, and a NaN or infinity in it reaches only the queries
+    that see its token.  `out` must not overlap q.  Workspace is cached per (device, stream, head_dim); calls
     on one stream run in order, so sharing it is safe."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if q.dim() != 3 or k_pool.dim() != 4:

@@ -438,7 +438,8 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * lse (nullable, fp32 [T,Hq]) = log sum exp(sm_scale q k); a query that sees no
  * key gets 0 and -inf.  Rows of q past cu_q[R] are left alone in out and lse.
  * Cache contents past kv_lens (the rest of the last page, other pages) are never
- * used, whatever they hold.
+ * used, whatever they hold; a NaN or infinity in the cache reaches only the
+ * queries that see its token.  out must not overlap q.
  * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
  * every pointer and stride of q, k_pool, v_pool and out a multiple of 16 bytes
  * (else FADE_ERR_ALIGN), 0 < sm_scale <= 1e30. */

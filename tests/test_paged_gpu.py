@@ -795,3 +795,11 @@ def test_chunk_attention_masked_values(cuda_device, new, kv, hq, hkv, D, page, d
     assert torch.equal(~lse.isinf(), some) and ((lse.double() - ref_lse).abs() <= lim_lse)[some].all()
     again = chunk_attention(q, kp, clean, table, cu, kl, causal=causal, window=window)   # nothing stays behind
     assert again.isfinite().all() and ((again.double() - ref).abs() <= lim).all()
+
+
+def test_chunk_attention_refuses_to_overwrite_q(cuda_device):
+    from fade_b200.paged import chunk_attention
+
+    args = _attn_inputs([3, 2], [30, 20], 4, 2, 64, 16, BF, cuda_device, 17)
+    with pytest.raises(ValueError):
+        chunk_attention(*args, out=args[0])
