@@ -1226,13 +1226,14 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     if (bad != FADE_OK) return bad;
     if (d->T == 0 || d->R == 0) return FADE_OK;
     if (!d->q || !d->out || !d->cu_q || !d->kv_lens || (d->table_width > 0 && !d->block_table) ||
-        (d->n_pages > 0 && (!d->k_pool || !d->v_pool)) || d->out == d->q)
+        (d->n_pages > 0 && (!d->k_pool || !d->v_pool)))
         return FADE_ERR_INVALID_ARG;
     const int64_t strides[] = {d->q_st, d->q_sh, d->o_st, d->o_sh, d->kp_sp, d->kp_sh, d->kp_st, d->vp_sp, d->vp_sh, d->vp_st};
     for (int64_t s : strides)
         if (s % 8) return FADE_ERR_ALIGN;
     if (!aligned16(d->q) || !aligned16(d->out) || !aligned16(d->k_pool) || !aligned16(d->v_pool)) return FADE_ERR_ALIGN;
     if (!workspace || ws_bytes < fade_chunk_attn_workspace_size(d)) return FADE_ERR_WORKSPACE;
+    if (d->out == d->q) return FADE_ERR_INVALID_ARG;
     const int G = fade_sm_count();
     if (G <= 0) return FADE_ERR_CUDA;
     ChunkParams p = {};
