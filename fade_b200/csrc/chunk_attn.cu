@@ -970,7 +970,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 
 // A warp looks again at the output of one row, which sees the keys [kmin, kend)
 // of the [lo, hi) that its tile went through.  If it is not finite and a V of
-// the tile's other keys is not, it is computed anew.
+// the tile's other keys is not, it is computed anew; from its last key, because
+// a request gone bad is bad from some token on, and with every channel in
+// question reached by a key that the row does see (or by a score), the row
+// stays as it is.
 template <int DT, int D>
 __device__ __forceinline__ void mend_row(const ChunkParams& p, int b, int h, int hq, int64_t t, int kmin, int kend, int lo,
                                       int hi) {
@@ -1001,9 +1004,13 @@ __device__ __forceinline__ void mend_row(const ChunkParams& p, int b, int h, int
     if (!__any_sync(~0u, bad)) return;
     const T* qp = static_cast<const T*>(p.q) + t * p.q_st + (int64_t)hq * p.q_sh + lane * N;
     float m = -INFINITY, l = 0.f, acc[N], q[N];
+    uint32_t open = 0;                                     // channels not finite, no such V seen yet
 #pragma unroll
-    for (int c = 0; c < N; ++c) acc[c] = 0.f, q[c] = Elem<DT>::to_f(qp[c]);
-    for (int j = kmin; j < kend; ++j) {
+    for (int c = 0; c < N; ++c) {
+        acc[c] = 0.f, q[c] = Elem<DT>::to_f(qp[c]);
+        if (!isfinite(Elem<DT>::to_f(out[c]))) open |= 1u << c;
+    }
+    for (int j = kend - 1; j >= kmin; --j) {
         const int64_t id = row[j >> p.page_log2];
         const bool in = id >= 0 && id < p.n_pages;         // beyond the pool: zeros
         float s = 0.f, v[N];
@@ -1015,6 +1022,10 @@ __device__ __forceinline__ void mend_row(const ChunkParams& p, int b, int h, int
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
         s *= p.scale_log2;
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            if (!isfinite(v[c])) open &= ~(1u << c);
+        if (s != s || !__any_sync(~0u, open != 0)) return;
         const float mn = fmaxf(m, s), off = mn == -INFINITY ? 0.f : mn;
         const float a = ex2(m - off), w = ex2(s - off);
         m = mn;

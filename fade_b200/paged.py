@@ -312,11 +312,12 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     Returns [T, Hq, D] (zeros where no key is visible; tokens past cu_q[R] are
     not written); with ``return_lse`` a dict of that as "out" and the float32
     [T, Hq] log of the sum of exponentials as "lse" (-inf where no key is
-    visible).  Head_dim 64 or 128, page
-    size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
-    kv_len is never used, and a NaN or infinity in it reaches only the queries
-    that see its token.  `out` must not overlap q.  Workspace is cached per (device, stream, head_dim); calls
-    on one stream run in order, so sharing it is safe."""
+    visible).  Head_dim 64 or 128, page size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
+    kv_len is never used, and a NaN or infinity in a token's K or V reaches only
+    the queries that see the token.  `out` must not overlap q.  Workspace is cached per
+    (device, stream, head_dim); calls on one stream run in order, so sharing it is
+    safe.  Graphs captured on one stream share it too: replay them in order, and
+    call once on that stream before the first capture."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if q.dim() != 3 or k_pool.dim() != 4:
         raise ValueError(f"q must be [tokens, heads, head_dim] and k_pool [pages, heads, page size, head_dim], got "
