@@ -451,11 +451,18 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         }
         return c;
     };
+    // prefix sums within the warps, where the first Q tile comes later
+    int64_t* scan = reinterpret_cast<int64_t*>(smem + L::Q_OFF);
     {
         int64_t c = cost_of(tid * per, per);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(~0u, c, o);
-        if (lane == 0) sums[warp] = c;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(~0u, c, o);
+            if (lane >= o) c += v;
+        }
+        scan[tid] = c;
+        if (lane == 31) sums[warp] = c;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
@@ -664,21 +671,18 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 int64_t at = 0;
                 int w = 0;
                 for (; w + 1 < kCaThreads / 32 && walk.x0 >= at + sums[w] * p.Hkv; ++w) at += sums[w] * p.Hkv;
-                const int64_t mine = cost_of((w * 32 + lane) * per, per) * p.Hkv;
-                int64_t incl = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t v = __shfl_up_sync(~0u, incl, o);
-                    if (lane >= o) incl += v;
-                }
+                const int64_t incl = scan[w * 32 + lane] * p.Hkv;
                 const int who = __ffs(__ballot_sync(~0u, walk.x0 < at + incl)) - 1;
-                at += __shfl_sync(~0u, incl - mine, who);
+                const int64_t before = who > 0 ? scan[w * 32 + who - 1] : 0, here = scan[w * 32 + who] - before;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                at += before * p.Hkv;
                 walk.b = (w * 32 + who) * per;
                 int64_t c;
                 for (;; ++walk.b) {
                     walk.r = load_req(p, walk.b);
                     walk.nt = tiles_of(p, walk.r);
-                    c = tiles_cost(p, walk.r, walk.nt, walk.nt);
+                    c = per == 1 ? here : tiles_cost(p, walk.r, walk.nt, walk.nt);
                     if (walk.x0 < at + c * p.Hkv || walk.b + 1 >= p.R) break;
                     at += c * p.Hkv;
                 }
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     span = min(step, span - k * step);
                     walk.i += k * step;
                 }
-                walk.pos = at + tiles_cost(p, walk.r, walk.i, walk.nt);
+                walk.pos = at + (walk.i > 0 ? tiles_cost(p, walk.r, walk.i, walk.nt) : 0);
             }
             if (lane == 0) {
                 *reinterpret_cast<Walk*>(smem + L::WALK_OFF) = walk;
