@@ -94,7 +94,7 @@ struct ChunkParams {
     int4* rec;          // [CTA][2]: the tile that begins in the CTA and crosses a cut; rows to look at again
     Walk* walks;        // [CTA]: the walk of its tiles, where rows are to be looked at again
     float2* part_ml;    // [CTA][continued tile, begun tile][256]: (maximum in the log2 domain, sum)
-    float4* part_o;     // [CTA][2][D / 4][256]
+    float4* part_o;     // [CTA][2][D / 8][256][2]
     const void *q, *k_pool, *v_pool;
     int64_t table_stride, o_st, o_sh, q_st, q_sh, kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
     uint32_t tile_magic;   // division by the tokens of a tile
@@ -942,11 +942,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                         for (int j = 0; j < 16; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
 #pragma unroll
                         for (int j = 0; j < 16; j += 8) st_row32(orow_p + c + 2 * j, y, j, p.out32);
-                    } else if (valid) {   // [channel / 4][row][4]: consecutive rows next to each other
+                    } else if (valid) {   // [channel / 8][row][8]: consecutive rows next to each other
+                        uint32_t y[32];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            p.part_o[((int64_t)slot * (D / 4) + c / 4 + j) * 256 + prow] =
-                                make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                        for (int j = 0; j < 32; ++j) y[j] = __float_as_uint(f[j]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            st_row32(p.part_o + (((int64_t)slot * (D / 8) + c / 8 + j) * 256 + prow) * 2, y, 8 * j, 1);
                     }
                     __syncwarp();
                 }
@@ -1110,7 +1112,13 @@ __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __gri
             const float2 ml = p.part_ml[slot * 256 + row];
             float4 v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = p.part_o[((int64_t)slot * (D / 4) + c4 + j) * 256 + row];
+            for (int j = 0; j < 4; j += 2) {
+                const float4* src = p.part_o + (((int64_t)slot * (D / 8) + (c4 + j) / 2) * 256 + row) * 2;
+                asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=f"(v[j].x), "=f"(v[j].y), "=f"(v[j].z), "=f"(v[j].w), "=f"(v[j + 1].x),
+                               "=f"(v[j + 1].y), "=f"(v[j + 1].z), "=f"(v[j + 1].w)
+                             : "l"(src));
+            }
             const float mn = fmaxf(m, ml.x);
             const float a = m == mn ? 1.f : ex2(m - mn), b = ml.x == -INFINITY ? 0.f : ex2(ml.x - mn);
             m = mn;
@@ -1249,6 +1257,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     if (!aligned16(d->q) || !aligned16(d->out) || !aligned16(d->k_pool) || !aligned16(d->v_pool)) return FADE_ERR_ALIGN;
     if (!workspace || ws_bytes < fade_chunk_attn_workspace_size(d)) return FADE_ERR_WORKSPACE;
     if (d->out == d->q) return FADE_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(workspace) % 32) return FADE_ERR_ALIGN;   // 32-byte loads and stores of the parts
     const int G = fade_sm_count();
     if (G <= 0) return FADE_ERR_CUDA;
     ChunkParams p = {};

@@ -457,8 +457,8 @@ typedef struct fade_chunk_desc {
     const int32_t* kv_lens;
 } fade_chunk_desc;
 
-/* Bytes of workspace fade_chunk_attn needs for `d` (0: unsupported).  Zero-fill
- * it once when allocating it; fade_workspace_check reads its error word. */
+/* Bytes of workspace fade_chunk_attn needs for `d` (0: unsupported), 32-byte
+ * aligned.  Zero-fill it once when allocating it; fade_workspace_check reads its error word. */
 size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d);
 int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream);
 
