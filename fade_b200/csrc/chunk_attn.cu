@@ -40,10 +40,11 @@
 //     - maximum - weights - weights x V are of one length.  Without turns
 //     1026 us; half of the exponentials on the FMA pipe instead (twelve
 //     instructions a pair) 995 us against 930 without.
-//   - 16 decodes of up to 8192 tokens: 76 us, 5.2 TB/s: HBM while it streams
+//   - 16 decodes of up to 8192 tokens: 74.5 us, 5.3 TB/s: HBM while it streams
 //     (5 TMA stages of 32 KB), the rest is start (5 us) and join (4 us).
-//   - 4 chunks of 1021 tokens, window 1024 (fp16): 101 us, 0.67 PFLOP/s: ten
+//   - 4 chunks of 1021 tokens, window 1024 (fp16): 100 us, 0.69 PFLOP/s: ten
 //     blocks a tile, 2.5 us of output a tile, 10 us of joining.
+//
 // V of masked keys.  A weight of zero times a NaN or an infinity is NaN in the
 // tensor core, so a V that only some rows of a tile see would reach them all.
 // The output of a tile is checked as it is written; rows that are not finite
@@ -1084,9 +1085,11 @@ __device__ __forceinline__ void mend(const ChunkParams& p, int c, int rows) {
 // block per CTA of the first kernel and slice of rows; a thread per row and
 // sixteen channels (four loads a part in flight, 32 bytes stored), rows
 // fastest, so that a warp reads neighbouring rows.
-// Mending is inlined and capped at three blocks per SM: as calls it needs a
-// stack, and 16 decodes take 76.3 us against 75.6 (74.0 without it); without
-// the cap 77.3.
+// Mending is inlined and capped at three blocks per SM (80 registers): when it
+// was added, 16 decodes went from 74.0 to 75.6 us; as calls, which need a stack,
+// to 76.3, without the cap to 77.3.  A second loop for few rows, with less per
+// thread and more parts in flight, costs more in cold instructions than it
+// saves (75.6 against 74.4).
 constexpr int kJoinThreads = 256;
 
 template <int DT, int D>
