@@ -228,6 +228,7 @@ _SIGNATURES = {
     "fade_rope_axes": (ctypes.c_int, [_vp, _vp]),
     "fade_chunk_attn_workspace_size": (ctypes.c_size_t, [_vp]),
     "fade_chunk_attn": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "fade_set_wait_polls": (ctypes.c_int, [_c_i64]),
 }
 
 _lib = None

@@ -80,7 +80,7 @@ constexpr int kTileCost = 384;
 constexpr int kMinShare = 384;         // least work of a CTA: a block per stream, and a block of any tile
 static_assert(kMinShare >= kCostTwo * kBlk, "every cut past a tile's start must move it by a block");
 constexpr float kLazyMax = 8.f;        // weights may grow to 2^8 before the maximum is moved
-constexpr uint32_t kCaPolls = 1u << 22;
+constexpr uint32_t kCaPolls = 1u << 22;   // polls of a wait before it gives up, unless the host asks for fewer
 constexpr uint32_t kSegPolls = 1u << 26;
 
 struct Walk;
@@ -102,6 +102,7 @@ struct ChunkParams {
     int tile_shift;
     int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32;
     float scale_log2, lazy;   // lazy: how far a score may exceed the running maximum
+    uint32_t polls;           // of a wait before it gives up
 };
 
 // ---------------------------------------------------------------------------
@@ -236,14 +237,29 @@ struct Walk {
 // ---------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ bool ca_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* err) {
-    for (uint32_t i = 0; i < kCaPolls; ++i) {
+// Waits are bounded.  One that runs out sets the CTA's flag and the error word,
+// and every other wait of the CTA gives up after it.  The lanes of a warp may
+// see that at different polls, so a warp goes on or stops by a vote of its
+// lanes; a warp that stops starts no more copies or products, waits for those
+// it has started (settle) and meets the others at the end of the kernel.
+__device__ __forceinline__ bool ca_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const ChunkParams& p) {
+    for (uint32_t i = 0; i < p.polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 255u && *abort_flag) return false;
     }
     *abort_flag = 1;
-    atomicExch(err, 1);
+    atomicExch(p.err, 1);
     return false;
+}
+// the same answer for the whole warp
+__device__ __forceinline__ bool ca_wait_all(uint32_t bar, uint32_t parity, volatile int* abort_flag, const ChunkParams& p) {
+    return __all_sync(~0u, ca_wait(bar, parity, abort_flag, p));
+}
+// For what this warp has started itself: it ends by itself, given up or not.
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity, const ChunkParams& p) {
+    for (uint32_t i = 0; i < kCaPolls; ++i)
+        if (mbar_try_wait(bar, parity)) return;
+    atomicExch(p.err, 1);
 }
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
@@ -367,7 +383,7 @@ struct CaLayout {
     static constexpr int NS = D == 128 ? 5 : 11;           // ring stages, one K or V block each
     static constexpr int ML_OFF = RING_OFF + NS * TILE;    // (m, l) of both streams
     static constexpr int BAR_OFF = ML_OFF + 2 * 128 * 8;
-    static constexpr int N_BARS = 2 * NS + 21 + 2 * kSegSlots;
+    static constexpr int N_BARS = 2 * NS + 23 + 2 * kSegSlots;
     static constexpr int MISC_OFF = BAR_OFF + 8 * N_BARS;  // tensor-memory slot, abort flag, output not finite
     static constexpr int SEG_OFF = (MISC_OFF + 16 + 15) / 16 * 16;
     static constexpr int SUM_OFF = SEG_OFF + kSegSlots * (int)sizeof(Seg);   // costs per warp
@@ -406,6 +422,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     auto h_full = [&](int x) { return b1 + 8u * (11 + 2 * kSegSlots + x); };   // weights of the block's first half
     auto turn = [&](int x, int w) { return b1 + 8u * (13 + 2 * kSegSlots + 4 * x + w); };   // warp w of stream x may take exponentials
 
+    auto done = [&](int x) { return b1 + 8u * (21 + 2 * kSegSlots + x); };   // products of stream x, when its MMA warp ends
+
     if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
         if (tid == 0) {
             atomicExch(p.err, 1);
@@ -426,6 +444,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             mbar_init(p_full(x), 4);
             mbar_init(h_full(x), 4);
             mbar_init(o_full(x), 1);
+            mbar_init(done(x), 1);
         }
         mbar_init(both, 8);
         for (int i = 0; i < 8; ++i) mbar_init(turn(i / 4, i % 4), 1);
@@ -476,7 +495,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
     uint32_t seg_phase = 0;
     // the next posted segment; every lane reads it, one says so
     auto next_seg = [&] {
-        const bool ok = ca_wait(seg_full(seg), seg_phase, abort_flag, p.err);
+        const bool ok = ca_wait_all(seg_full(seg), seg_phase, abort_flag, p);
         s = segs[seg];
         __syncwarp();
         if (lane == 0) mbar_arrive(seg_empty(seg));
@@ -501,11 +520,13 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             uint32_t q_phase = 3;   // bit x: parity to wait for on buffer x
             int flip = 0, stage = 0;
             uint32_t phase = 1;
-            while (next_seg()) {
+            bool run = true;
+            while (run && next_seg()) {
                 if (s.k1 == s.k0) continue;
                 const bool two = s.n > p.tq;
                 for (int x = two ? 0 : flip; x < (two ? 2 : flip + 1); ++x) {
-                    ca_wait(q_empty(x), (q_phase >> x) & 1u, abort_flag, p.err);
+                    run = ca_wait_all(q_empty(x), (q_phase >> x) & 1u, abort_flag, p);
+                    if (!run) break;
                     q_phase ^= 1u << x;
                     if (lane == 0) {
                         mbar_arrive_tx(q_full(x), 128u * (D / 64) * p.g * p.tq);
@@ -524,7 +545,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 };
                 int base = s.k0 * ppb & ~31;
                 int cur = entry(base + lane), nxt = entry(base + 32 + lane);
-                for (int kb = s.k0; kb < s.k1; ++kb) {
+                for (int kb = s.k0; run && kb < s.k1; ++kb) {
                     if (kb * ppb >= base + 32) {
                         base += 32;
                         cur = nxt;
@@ -533,7 +554,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     const int id = __shfl_sync(~0u, cur, (kb * ppb + my_page) & 31);
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv) {
-                        ca_wait(empty(stage), phase, abort_flag, p.err);
+                        run = ca_wait_all(empty(stage), phase, abort_flag, p);
+                        if (!run) break;
                         if (lane == 0) mbar_arrive_tx(full(stage), L::TILE);
                         __syncwarp();
                         if (my_sub < D / 64)
@@ -543,9 +565,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     }
                 }
             }
-            // every copy has landed before the CTA may exit
+            // every copy has landed before the CTA may exit, and where nothing gave up has been used
+            for (int i = 0; i < L::NS; ++i) settle(full(i), i < stage ? phase ^ 1u : phase, p);
+            for (int x = 0; x < 2; ++x) settle(q_full(x), (q_phase >> x) & 1u, p);
             for (int i = 0; i < L::NS; ++i) {
-                ca_wait(empty(stage), phase, abort_flag, p.err);
+                ca_wait(empty(stage), phase, abort_flag, p);
                 if (++stage == L::NS) stage = 0, phase ^= 1u;
             }
         } else if (warp == 9 || warp == 11) {
@@ -557,7 +581,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             // where only the other one uses it (two arrivals free a buffer):
             // a warp that skipped fills could mistake one for another.
             const int st = warp == 9 ? 0 : 1;
-            const bool lead = elect_one();
+            const bool elected = elect_one();
+            bool run = true, lead = elected;     // lead: this lane issues
             constexpr uint32_t IQK = ca_idesc<DT>(kBlk, false), IPV = ca_idesc<DT>(D, true);
             const uint64_t q_desc = tc_desc(sb + L::Q_OFF, 16, 1024, 2);
             const uint64_t k_desc = tc_desc(sb + L::RING_OFF, 16, 1024, 2);
@@ -566,7 +591,11 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             uint32_t q_phase = 0, p_phase = 0;   // bit x of q_phase: parity to wait for on buffer x
             int flip = 0, stage = 0;             // next ring stage: K, V, K, V, ... of the blocks
             uint32_t phase = 0;
-            auto landed = [&] { ca_wait(full(stage), phase, abort_flag, p.err); };
+            auto wait = [&](uint32_t bar, uint32_t parity) {
+                run = run && ca_wait_all(bar, parity, abort_flag, p);
+                lead = elected && run;
+            };
+            auto landed = [&] { wait(full(stage), phase); };
             auto advance = [&] {
                 if (++stage == L::NS) stage = 0, phase ^= 1u;
             };
@@ -578,12 +607,12 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 }
                 __syncwarp();
             };
-            while (next_seg()) {
+            while (run && next_seg()) {
                 const int nb = s.k1 - s.k0;
                 if (nb == 0) continue;
                 const bool two = s.n > p.tq;
-                if (two || flip == 0) ca_wait(q_full(0), q_phase & 1u, abort_flag, p.err);
-                if (two || flip == 1) ca_wait(q_full(1), q_phase >> 1, abort_flag, p.err);
+                if (two || flip == 0) wait(q_full(0), q_phase & 1u);
+                if (two || flip == 1) wait(q_full(1), q_phase >> 1);
                 const int x = two ? st : flip;   // Q buffer
                 q_phase ^= two ? 3u : 1u << flip;
                 if (!two) flip ^= 1;
@@ -610,14 +639,14 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     __syncwarp();
                     advance();
                 }
-                for (int j = 0; j < mine; ++j) {
+                for (int j = 0; run && j < mine; ++j) {
                     const bool more = j + 1 < mine, now = two && more;   // the next scores follow at once
                     landed();
                     const uint64_t b = v_desc + (uint32_t)(stage * (L::TILE >> 4));
                     const uint32_t v_empty = empty(stage);
                     advance();
                     if (now) landed();
-                    ca_wait(h_full(st), p_phase, abort_flag, p.err);
+                    wait(h_full(st), p_phase);
                     tc_fence_after();
                     if (lead) {
                         tc_mma_ts(to, ts, b, IPV, j > 0 ? 1u : 0u);
@@ -625,7 +654,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                         for (int i = 1; i < kBlk / 32; ++i) tc_mma_ts(to, ts + 8 * i, b + (uint32_t)(i * 128), IPV, 1u);
                     }
                     __syncwarp();
-                    ca_wait(p_full(st), p_phase, abort_flag, p.err);
+                    wait(p_full(st), p_phase);
                     p_phase ^= 1u;
                     tc_fence_after();
                     if (lead) {
@@ -650,6 +679,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     }
                 }
             }
+            // the products have ended before tensor memory is given back and the CTA exits
+            if (elected) tc_commit(done(st));
+            __syncwarp();
+            settle(done(st), 0, p);
         } else if (warp == 10) {
             // ------------------------ tiles, in order ------------------------
             // Range of this CTA: [x0, x1) of the total cost W, of which the
@@ -702,20 +735,22 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             }
             if (lane == 0) {
                 *reinterpret_cast<Walk*>(smem + L::WALK_OFF) = walk;
-                bool more = true;
+                bool more = true, run = true;
                 while (more) {
                     more = walk.next(p, s);
                     if (!more) s.n = 0;
                     // a segment may take long: look for a free slot now and then
-                    for (uint32_t i = 0; i < kSegPolls && !mbar_try_wait(seg_empty(seg), seg_phase ^ 1u); ++i) {
-                        if (*abort_flag) break;
+                    for (uint32_t i = 0; run && !mbar_try_wait(seg_empty(seg), seg_phase ^ 1u); ++i) {
                         if (i + 1 == kSegPolls) *abort_flag = 1, atomicExch(p.err, 1);
+                        run = !*abort_flag;
                         __nanosleep(200);
                     }
+                    if (!run) break;   // the slot may be in use
                     segs[seg] = s;
                     mbar_arrive(seg_full(seg));
                     if (++seg == kSegSlots) seg = 0, seg_phase ^= 1u;
                 }
+                if (!run) walk.parts_from = walk.parts_to = 0;
                 p.rec[cta * 2] = make_int4(walk.parts_from, walk.parts_to, walk.parts_n, walk.parts_tok);
                 p.rec[cta * 2 + 1] = make_int4(walk.parts_h, 0, walk.parts_b, 0);
             }
@@ -735,7 +770,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         auto meet = [&] {   // a bounded wait, so that no warp is left behind when another gave up
             __syncwarp();
             if (lane == 0) mbar_arrive(both);
-            ca_wait(both, meetings & 1u, abort_flag, p.err);
+            ca_wait(both, meetings & 1u, abort_flag, p);
             ++meetings;
             __syncwarp();
         };
@@ -746,10 +781,10 @@ __global__ void __launch_bounds__(kCaThreads, 1)
         };
         while (true) {
             // the segment stays in its slot until this warp is through with it
-            ca_wait(seg_full(seg), seg_phase, abort_flag, p.err);
+            if (!ca_wait_all(seg_full(seg), seg_phase, abort_flag, p)) break;
             const Seg& g = segs[seg];
             const int n = g.n;
-            if (n <= 0 || *abort_flag) break;
+            if (n <= 0) break;
             const bool two = n > p.tq;
             const int k0 = g.k0, k1 = g.k1;
             const int t = (two ? st * p.tq : 0) + tok;                // token within the tile
@@ -757,6 +792,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             const bool warp_on = __any_sync(~0u, valid);
             float m = -INFINITY, l = 0.f;
             int blocks = 0;
+            bool ok = true;
             {
                 // keys of this row: [kmin, kend); blocks that every row of the half tile sees whole: [free0, free1)
                 const int kv = g.kv, first = g.pos + (two ? st * p.tq : 0);
@@ -766,7 +802,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                 const int free0 = p.window > 0 ? (max(first + p.tq - p.window, 0) + kBlk - 1) / kBlk : 0;
                 const int step = two ? 1 : 2;
                 for (int kb = k0 + (two ? 0 : st); kb < k1; kb += step, ++blocks) {
-                    const bool ok = __all_sync(~0u, ca_wait(s_full(st), s_phase, abort_flag, p.err));
+                    ok = ca_wait_all(s_full(st), s_phase, abort_flag, p);
+                    if (!ok) break;
                     s_phase ^= 1u;
                     tc_fence_after();
                     // keys past the end of the cache: their V rows (the rest of a page) may hold anything
@@ -774,7 +811,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                         if (kb * kBlk + kBlk <= kv) return;
                         if (!two || st == 0) {
                             const uint32_t vp = ring + 2u * (kb - k0) + 1u;
-                            ca_wait(full(vp % L::NS), (vp / L::NS) & 1u, abort_flag, p.err);
+                            ca_wait(full(vp % L::NS), (vp / L::NS) & 1u, abort_flag, p);
                             const int keep = kv - kb * kBlk;
                             uint8_t* v = smem + L::RING_OFF + (vp % L::NS) * L::TILE;
                             for (int i = row; i < (kBlk - keep) * (D / 8); i += 128) {
@@ -790,7 +827,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     // half a block apart, so that one's MMAs run under the other's exponentials.
                     auto take_turn = [&] {
                         if (!two) return;
-                        ca_wait(my_turn, turn_phase, abort_flag, p.err);
+                        ca_wait(my_turn, turn_phase, abort_flag, p);
                         turn_phase ^= 1u;
                         __syncwarp();
                     };
@@ -802,7 +839,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar);
                     };
-                    if (!(warp_on && ok)) {
+                    if (!warp_on) {
                         clear_rest();
                         take_turn();
                         pass_turn();
@@ -882,6 +919,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     l += a + b;
                 }
             }
+            if (!ok) break;
             const int nb = k1 - k0;
             ring += 2u * nb;
             const int64_t orow = (int64_t)g.tok + t;
@@ -896,7 +934,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
             release();
             if (nb == 0) continue;
             if (blocks > 0) {
-                ca_wait(o_full(st), o_phase, abort_flag, p.err);
+                if (!ca_wait_all(o_full(st), o_phase, abort_flag, p)) break;
                 o_phase ^= 1u;
             }
             __syncwarp();
@@ -1155,6 +1193,8 @@ __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __gri
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
+static std::atomic<int64_t> g_wait_polls{kCaPolls};
+
 static PFN_cuTensorMapEncodeTiled_v12000 ca_encode_fn() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;
@@ -1309,6 +1349,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     p.out32 = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_st % 16 == 0 && d->o_sh % 16 == 0;
     p.scale_log2 = (float)(d->sm_scale * 1.4426950408889634);
     p.lazy = std::min(kLazyMax / p.scale_log2, 1e30f);   // finite: the first maximum always replaces -inf
+    p.polls = (uint32_t)g_wait_polls.load(std::memory_order_relaxed);
     CUtensorMap tq, tk, tv;
     const cuuint64_t qd[3] = {(cuuint64_t)d->D, (cuuint64_t)d->Hq, (cuuint64_t)d->T};
     const int64_t qs[2] = {d->q_sh, d->q_st};
@@ -1330,4 +1371,10 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
                           : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, s);
     return d->D == 64 ? launch_chunk<FADE_BF16, 64>(tq, tk, tv, p, G, s)
                       : launch_chunk<FADE_BF16, 128>(tq, tk, tv, p, G, s);
+}
+
+extern "C" int fade_set_wait_polls(int64_t polls) {
+    if (polls > kCaPolls) return FADE_ERR_INVALID_ARG;
+    g_wait_polls.store(polls < 0 ? kCaPolls : polls, std::memory_order_relaxed);
+    return FADE_OK;
 }

@@ -462,6 +462,13 @@ typedef struct fade_chunk_desc {
 size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d);
 int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream);
 
+/* Polls after which a device wait of later fade_chunk_attn calls gives up (the
+ * call then ends, its outputs are undefined and the workspace's error word is
+ * set): 0 to 2^22, the default; negative: the default again.  Process-wide.  A
+ * low number makes waits run out that would have ended, so that a host's handling
+ * of the error can be exercised. */
+int fade_set_wait_polls(int64_t polls);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,47 @@
+"""The paged serving step where things go wrong: waits that run out, threads,
+captured steps, strides that are never stepped, values at the types' limits."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_paged_gpu import BF, HF, _attn_inputs, _attn_ref
+
+pytestmark = pytest.mark.gpu
+
+
+# (new, kv, hq, hkv, D, page, dtype): decodes over split tiles, chunks of two half tiles, both in one batch
+GIVE_UP = [
+    ([1, 1, 5], [3000, 700, 900], 8, 2, 128, 32, BF),
+    ([300], [2000], 8, 2, 64, 64, HF),
+    ([260, 1, 0, 3], [1500, 4000, 9, 3], 28, 4, 128, 16, BF),
+]
+
+
+@pytest.mark.parametrize("polls", [0, 1, 3, 40, 1000])
+@pytest.mark.parametrize("new,kv,hq,hkv,D,page,dt", GIVE_UP)
+def test_waits_that_run_out_are_reported(cuda_device, polls, new, kv, hq, hkv, D, page, dt):
+    """A call whose device waits give up ends, says so, and leaves nothing behind for the next one."""
+    from fade_b200 import _lib
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    lib = _lib.load()
+    args = _attn_inputs(new, kv, hq, hkv, D, page, dt, cuda_device, 31)
+    clean = chunk_attention(*args)
+    check_device_errors(cuda_device)
+    ref, _, lim, _ = _attn_ref(*args[:4], new, kv, True, None, D ** -0.5)
+    for _ in range(5):
+        try:
+            assert lib.fade_set_wait_polls(polls) == _lib.FADE_OK
+            out = chunk_attention(*args)
+        finally:
+            assert lib.fade_set_wait_polls(-1) == _lib.FADE_OK
+        try:
+            check_device_errors(cuda_device)
+            assert polls > 0 and ((out.double() - ref).abs() <= lim).all()
+        except RuntimeError as e:
+            assert "timed out" in str(e)
+        check_device_errors(cuda_device)                          # reported once
+        assert torch.equal(chunk_attention(*args), clean)
+        check_device_errors(cuda_device)
