@@ -1236,11 +1236,12 @@ static int make_map(CUtensorMap* m, int dtype, const void* base, int rank, const
         if (strides[i] < 0) return FADE_ERR_INVALID_ARG;
         bytes[i] = (cuuint64_t)strides[i] * 2;
     }
-    const CUresult r = enc(m, dtype == FADE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                           rank, const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? FADE_OK : FADE_ERR_ALIGN;
+    const bool ok = encoded([&] {
+        return enc(m, dtype == FADE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                   const_cast<void*>(base), dims, bytes, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+    return ok ? FADE_OK : FADE_ERR_ALIGN;
 }
 
 constexpr int kWalkBytes = 128;   // of a CTA in the workspace

@@ -44,6 +44,15 @@ void set_last_cuda_error(int e);
         }                                            \
     } while (0)
 
+// Encodes a tensor map.  The driver call needs a current context, which a host
+// thread that has not used the GPU yet lacks (the runtime makes one current by
+// itself, but not for this): on failure once more behind a cudaSetDevice.
+template <class Encode> inline bool encoded(const Encode& encode) {
+    if (encode() == 0) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode() == 0;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -2231,10 +2231,12 @@ static int make_row_map(CUtensorMap* m, const void* base, int64_t n_rows, int ro
     cuuint64_t strides[1] = {128};
     cuuint32_t box[2] = {128, (cuuint32_t)(kStageTokens * row_bytes / 128)};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
-                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? FADE_OK : FADE_ERR_ALIGN;
+    const bool ok = encoded([&] {
+        return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+    return ok ? FADE_OK : FADE_ERR_ALIGN;
 }
 
 // V scales: per-token -> 1-D map over rows (box = one stage of rows);
@@ -2243,26 +2245,30 @@ static int make_row_map(CUtensorMap* m, const void* base, int64_t n_rows, int ro
 static int make_scale_map(CUtensorMap* m, const void* base, int64_t n_rows, bool grouped, int D, int G) {
     auto enc = encode_fn();
     if (!enc) return FADE_ERR_CUDA;
-    CUresult r;
+    bool ok;
     if (!grouped) {
         cuuint64_t dims[1] = {(cuuint64_t)n_rows};
         cuuint64_t strides[1] = {2};
         cuuint32_t box[1] = {(cuuint32_t)kStageTokens};
         cuuint32_t estr[1] = {1};
-        r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 1, const_cast<void*>(base), dims, strides + 1, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        ok = encoded([&] {
+            return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 1, const_cast<void*>(base), dims, strides + 1, box, estr,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        });
     } else {
         const int64_t n_groups = (n_rows + G - 1) / G;
         cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)n_groups};
         cuuint64_t strides[1] = {(cuuint64_t)D * 2};
         cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)(kStageTokens / G)};
         cuuint32_t estr[2] = {1, 1};
-        r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        ok = encoded([&] {
+            return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        });
     }
-    return r == CUDA_SUCCESS ? FADE_OK : FADE_ERR_ALIGN;
+    return ok ? FADE_OK : FADE_ERR_ALIGN;
 }
 
 static int sm_count() {

@@ -3,6 +3,8 @@ captured steps, strides that are never stepped, values at the types' limits."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
@@ -45,3 +47,39 @@ def test_waits_that_run_out_are_reported(cuda_device, polls, new, kv, hq, hkv, D
         check_device_errors(cuda_device)                          # reported once
         assert torch.equal(chunk_attention(*args), clean)
         check_device_errors(cuda_device)
+
+
+def _in_new_thread(work):
+    """work() in a thread that has not used the GPU."""
+    got = []
+
+    def loop():
+        try:
+            got.append(work())
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    t = threading.Thread(target=loop)
+    t.start()
+    t.join(timeout=60)
+    torch.cuda.synchronize()
+    assert got and not isinstance(got[0], Exception), got
+    return got[0]
+
+
+def test_first_call_of_a_thread(cuda_device):
+    """The tensor maps are made in a thread that has no context yet."""
+    from fade_b200.attention import Int4Tier, tiered_decode_attention
+    from fade_b200.paged import chunk_attention
+    from fade_b200.quant import quant_k_int4, quant_v_int4
+
+    args = _attn_inputs([3, 1], [900, 40], 8, 2, 64, 16, HF, cuda_device, 32)
+    want = chunk_attention(*args)
+    out = torch.zeros_like(want)                                  # (torch's own launches would make the context current)
+    assert torch.equal(_in_new_thread(lambda: chunk_attention(*args, out=out)), want)
+    g = torch.Generator(device="cuda").manual_seed(33)
+    k, v = (torch.randn(1, 2, 256, 128, generator=g, device=cuda_device).to(BF) for _ in range(2))
+    tier = Int4Tier(*quant_k_int4(k), *quant_v_int4(v))
+    q = torch.randn(1, 8, 1, 128, generator=g, device=cuda_device).to(BF)
+    want = tiered_decode_attention(q, [tier])
+    assert torch.equal(_in_new_thread(lambda: tiered_decode_attention(q, [tier])), want)
