@@ -6,6 +6,11 @@
 namespace fade {
 static std::atomic<int> g_last_cuda_error{0};
 void set_last_cuda_error(int e) { g_last_cuda_error.store(e); }
+
+std::mutex& workspace_mutex(const void* workspace) {
+    static std::mutex mu[64];   // workspaces that share one only wait a launch longer
+    return mu[(reinterpret_cast<uintptr_t>(workspace) >> 9) % 64];
+}
 }  // namespace fade
 
 extern "C" const char* fade_status_string(int status) {

@@ -1367,6 +1367,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
     if ((st = make_map(&tk, (int)d->dtype, kb, 4, kd, ks, kbox)) != FADE_OK) return st;
     if ((st = make_map(&tv, (int)d->dtype, vb, 4, kd, vs, kbox)) != FADE_OK) return st;
     cudaStream_t s = as_stream(stream);
+    std::lock_guard<std::mutex> lock(workspace_mutex(workspace));
     if (d->dtype == FADE_F16)
         return d->D == 64 ? launch_chunk<FADE_F16, 64>(tq, tk, tv, p, G, s)
                           : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, s);

@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/fade_b200.h"
 
 namespace fade {
@@ -52,6 +54,11 @@ template <class Encode> inline bool encoded(const Encode& encode) {
     int dev = 0;
     return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode() == 0;
 }
+
+// Held over the launches of a call that hands data from one kernel to the next
+// through `workspace`: calls of several host threads that share it on a stream
+// then follow one another whole, instead of launch by launch.
+std::mutex& workspace_mutex(const void* workspace);
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

@@ -315,8 +315,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     visible).  Head_dim 64 or 128, page size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
     kv_len is never used, and a NaN or infinity in a token's K or V reaches only
     the queries that see the token.  `out` must not overlap q.  Workspace is cached per
-    (device, stream, head_dim); calls on one stream run in order, so sharing it is
-    safe.  Graphs captured on one stream share it too: replay them in order, and
+    (device, stream, head_dim); calls on one stream, from any number of host
+    threads, follow one another whole, so sharing it is safe.  Graphs captured on one stream share it too: replay them in order, and
     call once on that stream before the first capture."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if q.dim() != 3 or k_pool.dim() != 4:
@@ -366,7 +366,7 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
         if need == 0:
             raise ValueError(f"unsupported chunk attention sizes (R={R}, T={T}, n_pages={n_pages}, table width {width})")
         ws = torch.zeros(need, dtype=torch.uint8, device=q.device)
-        _WS[(dev, st, D)] = ws = (ws, ws.data_ptr(), need)
+        ws = _WS.setdefault((dev, st, D), (ws, ws.data_ptr(), need))     # another thread's, if it was first
     code = lib.fade_chunk_attn(d, ws[1], ws[2], st)
     if code:
         _lib.check(code, "chunk_attention")

@@ -458,7 +458,9 @@ typedef struct fade_chunk_desc {
 } fade_chunk_desc;
 
 /* Bytes of workspace fade_chunk_attn needs for `d` (0: unsupported), 32-byte
- * aligned.  Zero-fill it once when allocating it; fade_workspace_check reads its error word. */
+ * aligned.  Zero-fill it once when allocating it; fade_workspace_check reads its
+ * error word.  Calls may share a workspace on one stream, from several host
+ * threads too; calls on different streams may not. */
 size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d);
 int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream);
 

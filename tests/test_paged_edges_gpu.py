@@ -83,3 +83,46 @@ def test_first_call_of_a_thread(cuda_device):
     q = torch.randn(1, 8, 1, 128, generator=g, device=cuda_device).to(BF)
     want = tiered_decode_attention(q, [tier])
     assert torch.equal(_in_new_thread(lambda: tiered_decode_attention(q, [tier])), want)
+
+
+def _in_threads(works, rounds, stream):
+    """Each work over and over in a thread of its own, all on one stream; their results in order."""
+    results, errors = [[] for _ in works], []
+    start = threading.Barrier(len(works))
+
+    def loop(i):
+        try:
+            with torch.cuda.stream(stream):
+                start.wait(timeout=30)
+                for _ in range(rounds):
+                    results[i].append(works[i]())
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(len(works))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(timeout=120)
+    torch.cuda.synchronize()
+    assert not errors and not any(t.is_alive() for t in threads), errors
+    return results
+
+
+@pytest.mark.parametrize("own_stream", [False, True])
+def test_chunk_attention_from_threads_on_one_stream(cuda_device, own_stream):
+    """Batches of other sizes from other threads on the same stream: each gets its own result, bit for bit."""
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    batches = [_attn_inputs(new, kv, 8, 2, 128, 32, BF, cuda_device, 40 + i) for i, (new, kv) in enumerate(
+        (([1, 1, 1], [5000, 900, 2000]), ([300], [2500]), ([40, 1, 70], [1000, 7000, 70]), ([1], [9000])))]
+    alone = [chunk_attention(*b, return_lse=True) for b in batches]
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream() if own_stream else torch.cuda.default_stream()
+    results = _in_threads([lambda b=b: chunk_attention(*b, return_lse=True) for b in batches], 60, stream)
+    with torch.cuda.stream(stream):
+        check_device_errors(cuda_device)
+    for want, got in zip(alone, results):
+        assert len(got) == 60
+        for g in got:
+            assert torch.equal(g["out"], want["out"]) and torch.equal(g["lse"], want["lse"])
