@@ -375,7 +375,8 @@ def tiered_decode_attention(q: Tensor, tiers: list, sm_scale: float | None = Non
     GQA: query head ``hq`` reads kv head ``hq // (Hq // Hkv)`` (transformers'
     ``repeat_kv`` convention).  Non-causal over the cached tokens, as a decode
     step is.  Workspace is cached per (device, stream); calls that share a
-    stream run in order, so sharing it is safe.
+    stream, from any number of host threads, follow one another whole, so
+    sharing it is safe.
     """
     dev = _lib.require_cuda(q)
     plan = DecodePlan(q, tiers, out=out, sm_scale=sm_scale, n_ctas=n_ctas, cu_units=cu_units,

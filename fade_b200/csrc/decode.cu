@@ -2539,6 +2539,7 @@ static int decode_attn_impl(const fade_decode_desc* d, const fade_age_out_desc* 
     const bool rot = has_mid && d->seg[pl.mid_idx].kind == FADE_SEG_ROT;
     float* qrot = reinterpret_cast<float*>(ws + pl.off_qrot);
     const float qk_scale = d->sm_scale * kLog2e;
+    std::lock_guard<std::mutex> lock(workspace_mutex(workspace));
 
     if (rot) {
         const bool f16 = d->dtype == FADE_F16, d64 = d->D == 64;

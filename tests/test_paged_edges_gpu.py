@@ -126,3 +126,23 @@ def test_chunk_attention_from_threads_on_one_stream(cuda_device, own_stream):
         assert len(got) == 60
         for g in got:
             assert torch.equal(g["out"], want["out"]) and torch.equal(g["lse"], want["lse"])
+
+
+def test_tiered_decode_attention_from_threads_on_one_stream(cuda_device):
+    """As above for the decode over tiers, whose kernels hand partials on through a workspace, too."""
+    from fade_b200.attention import FPTier, Int4Tier, tiered_decode_attention
+    from fade_b200.quant import quant_k_int4, quant_v_int4
+
+    g = torch.Generator(device="cuda").manual_seed(50)
+
+    def batch(B, n):
+        k, v, rk, rv = (torch.randn(B, 2, m, 128, generator=g, device=cuda_device).to(BF) for m in (n, n, 64, 64))
+        q = torch.randn(B, 8, 1, 128, generator=g, device=cuda_device).to(BF)
+        return q, [Int4Tier(*quant_k_int4(k), *quant_v_int4(v)), FPTier(rk, rv)]
+
+    batches = [batch(1, 8192), batch(6, 1024), batch(3, 3000 // 8 * 8)]
+    alone = [tiered_decode_attention(*b) for b in batches]
+    torch.cuda.synchronize()
+    results = _in_threads([lambda b=b: tiered_decode_attention(*b) for b in batches], 60, torch.cuda.default_stream())
+    for want, got in zip(alone, results):
+        assert len(got) == 60 and all(torch.equal(g, want) for g in got)
