@@ -296,30 +296,46 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-_tls = threading.local()
-
-
-def bind(device: torch.device) -> int:
-    """Make `device` current for the library; returns the current stream handle."""
-    lib = load()
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    if getattr(_tls, "dev", None) != idx:
-        check(lib.fade_set_device(idx), "fade_set_device")
-        _tls.dev = idx
-    return _stream(idx)
-
-
-# the current stream's handle, without the stream object where torch offers that
+# the current device and a device's current stream handle, without torch's wrappers where it offers that
+_current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda idx: torch.cuda.current_stream(idx).cuda_stream)
 
 
-def bind_index(idx: int) -> int:
-    """``bind`` for a device index."""
-    if getattr(_tls, "dev", None) != idx:
-        check(load().fade_set_device(idx), "fade_set_device")
-        _tls.dev = idx
+def _switch(idx: int) -> None:
+    torch.cuda.set_device(idx)
+    check(load().fade_set_device(idx), "fade_set_device")
+
+
+def bind(device: torch.device) -> int:
+    """Make `device` current, for good; returns its current stream handle."""
+    idx = device.index if device.index is not None else _current()
+    if _current() != idx:
+        _switch(idx)
     return _stream(idx)
+
+
+class on_device:
+    """``with on_device(dev) as stream``: `dev` is current inside, its current
+    stream's handle is given, and the caller's device is current again after.
+    What is current is asked for every time: torch changes it, too."""
+
+    __slots__ = ("idx", "before")
+
+    def __init__(self, device: torch.device | int):
+        self.idx = device if isinstance(device, int) else device.index
+
+    def __enter__(self) -> int:
+        self.before = _current()
+        if self.idx is None:
+            self.idx = self.before
+        if self.before != self.idx:
+            _switch(self.idx)
+        return _stream(self.idx)
+
+    def __exit__(self, *exc) -> None:
+        if self.before != self.idx:
+            _switch(self.before)
 
 
 def same_device(*tensors: torch.Tensor) -> int:

@@ -316,9 +316,8 @@ class DecodePlan:
         self.desc = d
         self.out = out
         self._keep = keep
-        lib = _lib.load()
-        _lib.bind(dev)
-        need = lib.fade_decode_attn_workspace_size(ctypes.byref(d))
+        with _lib.on_device(dev):
+            need = _lib.load().fade_decode_attn_workspace_size(ctypes.byref(d))
         if need == 0:
             raise ValueError(
                 f"unsupported decode configuration (D={D}, Hq/Hkv*n_q={Hq // Hkv * n_q}, dtype={dtype})"
@@ -349,15 +348,15 @@ class DecodePlan:
 
     def run(self) -> Tensor:
         lib = _lib.load()
-        st = _lib.bind(self.device)
-        _lib.check(lib.fade_decode_attn(ctypes.byref(self.desc), self.workspace.data_ptr(), self.ws_bytes, st),
-                   "fade_decode_attn")
+        with _lib.on_device(self.device) as st:
+            _lib.check(lib.fade_decode_attn(ctypes.byref(self.desc), self.workspace.data_ptr(), self.ws_bytes, st),
+                       "fade_decode_attn")
         return self.out
 
     def check_device_errors(self) -> None:
-        st = _lib.bind(self.device)
-        _lib.check(_lib.load().fade_workspace_check(self.workspace.data_ptr(), self.ws_bytes, st),
-                   "fade_decode_attn")
+        with _lib.on_device(self.device) as st:
+            _lib.check(_lib.load().fade_workspace_check(self.workspace.data_ptr(), self.ws_bytes, st),
+                       "fade_decode_attn")
 
 
 _WS: dict = {}

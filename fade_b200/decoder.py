@@ -62,16 +62,16 @@ def age_out_int4(ring_k: Tensor, ring_v: Tensor, mid_kq: Tensor, mid_vq: Tensor,
         if k_new.shape != (B, H, D) or v_new is None or v_new.stride() != k_new.stride() or k_new.stride(2) != 1:
             raise ValueError("k_new / v_new must be [B, H, D] with a shared layout")
         new_sb, new_sh = k_new.stride(0), k_new.stride(1)
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_age_out_int4(
-            ring_k.data_ptr(), ring_v.data_ptr(), _lib.dtype_code(ring_k.dtype), B, H, D, R,
-            ring_k.stride(0), ring_k.stride(1), int(ring_origin), mid_kq.data_ptr(), mid_vq.data_ptr(),
-            mid_vs.data_ptr(), ks.data_ptr(), mid_sb, mid_sh, mid_kq.shape[2], mid_len.data_ptr(),
-            _lib.ptr(k_new), _lib.ptr(v_new), new_sb, new_sh, st,
-        ),
-        "age_out_int4",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_age_out_int4(
+                ring_k.data_ptr(), ring_v.data_ptr(), _lib.dtype_code(ring_k.dtype), B, H, D, R,
+                ring_k.stride(0), ring_k.stride(1), int(ring_origin), mid_kq.data_ptr(), mid_vq.data_ptr(),
+                mid_vs.data_ptr(), ks.data_ptr(), mid_sb, mid_sh, mid_kq.shape[2], mid_len.data_ptr(),
+                _lib.ptr(k_new), _lib.ptr(v_new), new_sb, new_sh, st,
+            ),
+            "age_out_int4",
+        )
 
 
 class _Layer:
@@ -214,8 +214,11 @@ class TieredDecoder:
 
     # ------------------------------------------------------------------- step
     def _launch_all(self, layer_events: list | None = None, before=None, after=None) -> None:
+        with _lib.on_device(self.device) as st:
+            self._launch_layers(st, layer_events, before, after)
+
+    def _launch_layers(self, st: int, layer_events: list | None, before, after) -> None:
         lib = _lib.load()
-        st = _lib.bind(self.device)
         for i, ly in enumerate(self.layers):
             if before is not None:
                 before(i)

@@ -101,6 +101,9 @@ def plan_step(new_lens: Tensor, kv_lens: Tensor, block_table: Tensor, free_pages
     else:
         dev = _lib.same_device(new_lens, kv_lens, block_table, free_pages, n_free, out.cu_q, out.kv_lens, out.positions,
                                out.slots, out.n_free, out.status)
+    if dev != _lib._current():
+        with _lib.on_device(dev):
+            return plan_step(new_lens, kv_lens, block_table, free_pages, n_free, page_size, total, out)
     R, F = new_lens.numel(), free_pages.numel()
     total = int(total)
     if page_size < 1 or page_size & (page_size - 1) or page_size > 1 << 20:
@@ -123,8 +126,7 @@ def plan_step(new_lens: Tensor, kv_lens: Tensor, block_table: Tensor, free_pages
         R, total, page_size, width, stride, F, _int32(new_lens, (R,), "new_lens"), kv_in, bt,
         _int32(free_pages, (F,), "free_pages"), n_in, _int32(out.cu_q, (R + 1,), "out.cu_q"), kv_out,
         _int32(out.positions, (total,), "out.positions"), slots.data_ptr(), n_out, _int32(out.status, (1,), "out.status"))
-    st = _lib.bind_index(dev)
-    code = _lib.load().fade_plan_step(d, st)
+    code = _lib.load().fade_plan_step(d, _lib._stream(dev))
     if code:
         _lib.check(code, "plan_step")
     return out
@@ -150,9 +152,9 @@ def release_rows(rows: Tensor, kv_lens: Tensor, block_table: Tensor, page_size: 
         status = torch.empty(1, dtype=torch.int32, device=dev)
     args = (_int32(kv_lens, (R,), "kv_lens"), _int32(free_pages, (F,), "free_pages"), _int32(n_free, (1,), "n_free"),
             _int32(status, (1,), "status"))
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_release_rows(rows.data_ptr(), R, args[0], bt, width, stride, page_size, args[1], F,
-                                             args[2], args[3], st), "release_rows")
+    with _lib.on_device(dev) as st:
+        _lib.check(_lib.load().fade_release_rows(rows.data_ptr(), R, args[0], bt, width, stride, page_size, args[1], F,
+                                                 args[2], args[3], st), "release_rows")
     return status
 
 
@@ -224,6 +226,10 @@ def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, 
     ``round_tables`` rounds cos and sin through x's dtype first, as the tables
     of ``MRope.compute_cos_sin`` are.  ``out`` may be x itself."""
     dev = _lib.same_device(x, positions, inv_freq) if out is None else _lib.same_device(x, positions, inv_freq, out)
+    if dev != _lib._current():
+        with _lib.on_device(dev):
+            return rope_axes(x, positions, inv_freq, sections, interleaved=interleaved, inverse=inverse,
+                             round_tables=round_tables, out=out)
     if x.dim() != 3:
         raise ValueError(f"expected a [tokens, heads, head_dim] tensor, got shape {tuple(x.shape)}")
     T, H, D = x.shape
@@ -234,8 +240,7 @@ def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, 
         _lib.dtype_code(x.dtype), T, H, 0, D, rot, axes, *sec, interleaved, inverse, round_tables, p64, ps,
         positions.data_ptr(), inv_freq.data_ptr(), x.data_ptr(), x_st, x_sh, out.data_ptr(), o_st, o_sh,
         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    st = _lib.bind_index(dev)
-    code = _lib.load().fade_rope_axes(d, st)
+    code = _lib.load().fade_rope_axes(d, _lib._stream(dev))
     if code:
         _lib.check(code, "rope_axes")
     return out
@@ -261,6 +266,10 @@ def rope_append(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Te
     offset (``StepPlan.slots``).  Tokens with a slot outside the pool (padding:
     -1) are rotated but not written.  ``out`` may be q itself."""
     dev = _lib.same_device(q, k, v, positions, inv_freq, slots, k_pool, v_pool, q if out is None else out)
+    if dev != _lib._current():
+        with _lib.on_device(dev):
+            return rope_append(q, k, v, positions, inv_freq, sections, slots, k_pool, v_pool, interleaved=interleaved,
+                               round_tables=round_tables, out=out)
     if q.dim() != 3 or k.dim() != 3:
         raise ValueError(f"q and k must be [tokens, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
     T, Hq, D = q.shape
@@ -283,8 +292,7 @@ def rope_append(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Te
         _lib.dtype_code(dtype), T, Hq, Hkv, D, rot, axes, *sec, interleaved, 0, round_tables, p64, ps,
         positions.data_ptr(), inv_freq.data_ptr(), q.data_ptr(), q_st, q_sh, out.data_ptr(), o_st, o_sh,
         k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, slots.data_ptr(), page_size, shape[0], *kp, *vp)
-    st = _lib.bind_index(dev)
-    code = _lib.load().fade_rope_axes(d, st)
+    code = _lib.load().fade_rope_axes(d, _lib._stream(dev))
     if code:
         _lib.check(code, "rope_append")
     return out
@@ -319,6 +327,10 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     threads, follow one another whole, so sharing it is safe.  Graphs captured on one stream share it too: replay them in order, and
     call once on that stream before the first capture."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
+    if dev != _lib._current():
+        with _lib.on_device(dev):
+            return chunk_attention(q, k_pool, v_pool, block_table, cu_q, kv_lens, causal=causal, window=window,
+                                   sm_scale=sm_scale, out=out, return_lse=return_lse)
     if q.dim() != 3 or k_pool.dim() != 4:
         raise ValueError(f"q must be [tokens, heads, head_dim] and k_pool [pages, heads, page size, head_dim], got "
                          f"{tuple(q.shape)} and {tuple(k_pool.shape)}")
@@ -359,7 +371,7 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
         causal, window or 0, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh, 0 if lse is None else lse.data_ptr(),
         *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"), _int32(kv_lens, (R,), "kv_lens"))
     lib = _lib.load()
-    st = _lib.bind_index(dev)
+    st = _lib._stream(dev)
     ws = _WS.get((dev, st, D))
     if ws is None:
         need = lib.fade_chunk_attn_workspace_size(d)
@@ -376,13 +388,13 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
 def check_device_errors(device: torch.device | str = "cuda") -> None:
     """Raise if a bounded device wait of an earlier ``chunk_attention`` call on
     the current stream gave up (synchronises)."""
-    dev = torch.device(device).index
-    dev = torch.cuda.current_device() if dev is None else dev
-    st = _lib.bind_index(dev)
-    for key, (_, ptr, need) in list(_WS.items()):
-        if key[:2] == (dev, st):
-            status = _lib.load().fade_workspace_check(ptr, need, st)
-            _lib.check(status, "chunk_attention")
+    device = torch.device(device)
+    with _lib.on_device(device) as st:
+        dev = _lib._current()
+        for key, (_, ptr, need) in list(_WS.items()):
+            if key[:2] == (dev, st):
+                status = _lib.load().fade_workspace_check(ptr, need, st)
+                _lib.check(status, "chunk_attention")
 
 
 # ---------------------------------------------------------------------------

@@ -47,8 +47,8 @@ def _pack_int4_last_dim(q_int8: Tensor) -> Tensor:
     D = q.shape[-1]
     rows = q.numel() // D if D else 0
     out = _contig_out((*q.shape[:-1], D // 2), torch.uint8, dev)
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_pack_codes(q.data_ptr(), rows, D, 4, out.data_ptr(), st), "pack_int4")
+    with _lib.on_device(dev) as st:
+        _lib.check(_lib.load().fade_pack_codes(q.data_ptr(), rows, D, 4, out.data_ptr(), st), "pack_int4")
     return out
 
 
@@ -59,8 +59,8 @@ def _unpack_int4_last_dim(packed: Tensor) -> Tensor:
     Dh = p.shape[-1]
     rows = p.numel() // Dh if Dh else 0
     out = _contig_out((*p.shape[:-1], Dh * 2), torch.int8, dev)
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_unpack_codes(p.data_ptr(), rows, Dh * 2, 4, out.data_ptr(), st), "unpack_int4")
+    with _lib.on_device(dev) as st:
+        _lib.check(_lib.load().fade_unpack_codes(p.data_ptr(), rows, Dh * 2, 4, out.data_ptr(), st), "unpack_int4")
     return out
 
 
@@ -73,8 +73,8 @@ def _pack_int2_last_dim(q: Tensor) -> Tensor:
     D = qc.shape[-1]
     rows = qc.numel() // D if D else 0
     out = _contig_out((*qc.shape[:-1], D // 4), torch.uint8, dev)
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_pack_codes(qc.data_ptr(), rows, D, 2, out.data_ptr(), st), "pack_int2")
+    with _lib.on_device(dev) as st:
+        _lib.check(_lib.load().fade_pack_codes(qc.data_ptr(), rows, D, 2, out.data_ptr(), st), "pack_int2")
     return out
 
 
@@ -85,8 +85,8 @@ def _unpack_int2_last_dim(packed: Tensor) -> Tensor:
     Dq = p.shape[-1]
     rows = p.numel() // Dq if Dq else 0
     out = _contig_out((*p.shape[:-1], Dq * 4), torch.int8, dev)
-    st = _lib.bind(dev)
-    _lib.check(_lib.load().fade_unpack_codes(p.data_ptr(), rows, Dq * 4, 2, out.data_ptr(), st), "unpack_int2")
+    with _lib.on_device(dev) as st:
+        _lib.check(_lib.load().fade_unpack_codes(p.data_ptr(), rows, Dq * 4, 2, out.data_ptr(), st), "unpack_int2")
     return out
 
 
@@ -100,10 +100,10 @@ def _quant_int4(x: Tensor, per_channel: bool) -> tuple[Tensor, Tensor]:
     dt = _lib.dtype_code(x.dtype)
     packed = _contig_out((B, H, S, D // 2), torch.uint8, dev)
     scale = _contig_out((B, H, 1, D) if per_channel else (B, H, S, 1), x.dtype, dev)
-    st = _lib.bind(dev)
-    fn = _lib.load().fade_quant_int4_k if per_channel else _lib.load().fade_quant_int4_v
-    _lib.check(fn(x.data_ptr(), dt, _lib.view4(x), packed.data_ptr(), scale.data_ptr(), st),
-               "quant_int4")
+    with _lib.on_device(dev) as st:
+        fn = _lib.load().fade_quant_int4_k if per_channel else _lib.load().fade_quant_int4_v
+        _lib.check(fn(x.data_ptr(), dt, _lib.view4(x), packed.data_ptr(), scale.data_ptr(), st),
+                   "quant_int4")
     return packed, scale
 
 
@@ -137,14 +137,14 @@ def _quant_int2(x: Tensor, group_size: int, want_i8: bool, want_packed: bool):
     q8 = _contig_out((B, H, S, D), torch.int8, dev) if want_i8 else None
     qp = _contig_out((B, H, S, D // 4), torch.uint8, dev) if want_packed else None
     scale = _contig_out((B, H, G, D), x.dtype, dev)
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_quant_int2_grouped(
-            x.data_ptr(), dt, _lib.view4(x), group_size, _lib.ptr(q8), _lib.ptr(qp), scale.data_ptr(), st
-        ),
-        "quant_int2",
-        f"S={S} must be divisible by group_size={group_size}",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_quant_int2_grouped(
+                x.data_ptr(), dt, _lib.view4(x), group_size, _lib.ptr(q8), _lib.ptr(qp), scale.data_ptr(), st
+            ),
+            "quant_int2",
+            f"S={S} must be divisible by group_size={group_size}",
+        )
     return q8, qp, scale
 
 
@@ -176,12 +176,12 @@ def _dequant_call(codes: Tensor, bits: int, scale: Tensor, mode: int, group: int
     out = _contig_out((B, H, S, D), dtype, dev)
     sc = scale.to(dtype).contiguous()
     c = codes.contiguous()
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_dequant(c.data_ptr(), bits, sc.data_ptr(), mode, group, _lib.dtype_code(dtype),
-                                 B, H, S, D, out.data_ptr(), st),
-        "dequant",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_dequant(c.data_ptr(), bits, sc.data_ptr(), mode, group, _lib.dtype_code(dtype),
+                                     B, H, S, D, out.data_ptr(), st),
+            "dequant",
+        )
     return out
 
 

@@ -43,13 +43,13 @@ def rerope_gather(k: Tensor, v: Tensor | None, keep_idx: Tensor, cos_old: Tensor
 
     co, so = tab(cos_old, S), tab(sin_old, S)
     cn, sn = tab(cos_new, n), tab(sin_new, n)
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_rerope_gather(
-            k.data_ptr(), _lib.ptr(v), _lib.dtype_code(k.dtype), _lib.view4(k), keep.data_ptr(), n,
-            _lib.ptr(co), _lib.ptr(so), _lib.ptr(cn), _lib.ptr(sn), 1 if apply_rope else 0,
-            k_out.data_ptr(), _lib.ptr(v_out), st,
-        ),
-        "rerope_gather",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_rerope_gather(
+                k.data_ptr(), _lib.ptr(v), _lib.dtype_code(k.dtype), _lib.view4(k), keep.data_ptr(), n,
+                _lib.ptr(co), _lib.ptr(so), _lib.ptr(cn), _lib.ptr(sn), 1 if apply_rope else 0,
+                k_out.data_ptr(), _lib.ptr(v_out), st,
+            ),
+            "rerope_gather",
+        )
     return k_out, v_out

@@ -54,14 +54,14 @@ def _rot(x: Tensor, R: Tensor, bits: int, kind: int) -> tuple[Tensor, Tensor]:
     packed = torch.empty(B, H, S, _packed_last(D, bits), dtype=torch.uint8 if bits != 3 else torch.int8, device=dev)
     scale = torch.empty((B, H, 1, D) if kind == 0 else (B, H, S, 1), dtype=x.dtype, device=dev)
     ws = torch.empty(max(B * H * D * 4, 16), dtype=torch.uint8, device=dev) if kind == 0 else None
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_rotated_quant(
-            x.data_ptr(), _lib.dtype_code(x.dtype), _lib.view4(x), Rd.data_ptr(), bits, kind,
-            packed.data_ptr(), scale.data_ptr(), _lib.ptr(ws), 0 if ws is None else ws.numel(), st
-        ),
-        "rotated_quant",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_rotated_quant(
+                x.data_ptr(), _lib.dtype_code(x.dtype), _lib.view4(x), Rd.data_ptr(), bits, kind,
+                packed.data_ptr(), scale.data_ptr(), _lib.ptr(ws), 0 if ws is None else ws.numel(), st
+            ),
+            "rotated_quant",
+        )
     return packed, scale
 
 
@@ -82,12 +82,12 @@ def _rot_deq(packed: Tensor, scale: Tensor, R: Tensor, bits: int, dtype: torch.d
     Rd = R.to(device=dev, dtype=torch.float32).contiguous()
     out = torch.empty(B, H, S, D, dtype=dtype, device=dev)
     sc = scale.to(dtype).contiguous()
-    st = _lib.bind(dev)
-    _lib.check(
-        _lib.load().fade_rotated_dequant(packed.contiguous().data_ptr(), bits, sc.data_ptr(), mode, Rd.data_ptr(),
-                                         _lib.dtype_code(dtype), B, H, S, D, out.data_ptr(), st),
-        "rotated_dequant",
-    )
+    with _lib.on_device(dev) as st:
+        _lib.check(
+            _lib.load().fade_rotated_dequant(packed.contiguous().data_ptr(), bits, sc.data_ptr(), mode, Rd.data_ptr(),
+                                             _lib.dtype_code(dtype), B, H, S, D, out.data_ptr(), st),
+            "rotated_dequant",
+        )
     return out
 
 

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import pytest
+import torch
+
 from fade_b200 import _lib
 
 
@@ -12,3 +15,77 @@ def test_wait_polls_are_bounded():
         assert lib.fade_set_wait_polls(0) == lib.fade_set_wait_polls(1 << 22) == _lib.FADE_OK
     finally:
         assert lib.fade_set_wait_polls(-1) == _lib.FADE_OK
+
+
+class _Devices:
+    """Two devices: torch's calls and a library that records what is current when it is called."""
+
+    def __init__(self, monkeypatch):
+        self.now, self.seen = 0, []
+        monkeypatch.setattr(_lib, "_lib", self)
+        monkeypatch.setattr(_lib, "_current", lambda: self.now, raising=False)
+        monkeypatch.setattr(_lib, "_stream", lambda idx: 0)           # the default stream has the same handle on both
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.now)
+        monkeypatch.setattr(torch.cuda, "set_device", self._set)
+        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        monkeypatch.setattr(_lib, "same_device", lambda *t: 1)
+        monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cuda", 1))
+
+    def _set(self, idx):
+        self.now = torch.device("cuda", idx).index
+
+    def fade_set_device(self, idx):
+        self.now = idx
+        return _lib.FADE_OK
+
+    def fade_status_string(self, status):
+        return b"status"
+
+    def fade_chunk_attn_workspace_size(self, d):
+        self.seen.append(self.now)
+        return 256
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.seen.append(self.now)
+            return _lib.FADE_OK
+
+        if not name.startswith("fade_"):
+            raise AttributeError(name)
+        return call
+
+
+def test_bind_follows_the_current_device(monkeypatch):
+    """torch changes the current device between two calls for the same one."""
+    lib = _Devices(monkeypatch)
+    _lib.bind(torch.device("cuda", 1))
+    assert lib.now == 1
+    torch.cuda.set_device(0)                      # the end of a `with torch.cuda.device(1)`, say
+    _lib.bind(torch.device("cuda", 1))
+    assert lib.now == 1
+
+
+@pytest.mark.parametrize("op", ["plan_step", "release_rows", "rope_axes", "rope_append", "chunk_attention", "quant_k_int4"])
+def test_calls_run_on_their_tensors_device(monkeypatch, op):
+    """... and leave the caller's device current, whatever was current in between."""
+    from fade_b200 import paged, quant
+
+    lib = _Devices(monkeypatch)
+    monkeypatch.setattr(paged, "_WS", {})
+    monkeypatch.setattr(quant, "_contig_out", lambda shape, dtype, dev: torch.empty(shape, dtype=dtype))
+    i = torch.zeros(1, dtype=torch.int32)
+    x, pool = torch.zeros(1, 1, 64, dtype=torch.float16), torch.zeros(1, 1, 16, 64, dtype=torch.float16)
+    call = {
+        "plan_step": lambda: paged.plan_step(i, i, i[None], i, i, 16, 1,
+                                             out=paged.StepPlan.empty(1, 1, "cpu")),
+        "release_rows": lambda: paged.release_rows(i.bool(), i, i[None], 16, i, i, i.clone()),
+        "rope_axes": lambda: paged.rope_axes(x, i, torch.zeros(32)),
+        "rope_append": lambda: paged.rope_append(x, x, x, i, torch.zeros(32), None, i.long(), pool, pool),
+        "chunk_attention": lambda: paged.chunk_attention(x, pool, pool, i[None], torch.zeros(2, dtype=torch.int32), i),
+        "quant_k_int4": lambda: quant.quant_k_int4(x[None]),
+    }[op]
+    for _ in range(2):
+        lib.seen.clear()
+        call()
+        assert lib.seen and set(lib.seen) == {1}
+        assert lib.now == 0
