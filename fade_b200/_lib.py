@@ -228,6 +228,7 @@ _SIGNATURES = {
     "fade_rope_axes": (ctypes.c_int, [_vp, _vp]),
     "fade_chunk_attn_workspace_size": (ctypes.c_size_t, [_vp]),
     "fade_chunk_attn": (ctypes.c_int, [_vp, _vp, ctypes.c_size_t, _vp]),
+    "fade_chunk_attn_check": (ctypes.c_int, [_vp]),
     "fade_set_wait_polls": (ctypes.c_int, [_c_i64]),
 }
 
@@ -296,10 +297,12 @@ def require_cuda(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
-# the current device and a device's current stream handle, without torch's wrappers where it offers that
+# the current device, a device's current stream handle, and whether the current stream is being captured,
+# without torch's wrappers where it offers that
 _current = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda idx: torch.cuda.current_stream(idx).cuda_stream)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None) or torch.cuda.is_current_stream_capturing
 
 
 def _switch(idx: int) -> None:

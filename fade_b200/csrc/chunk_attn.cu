@@ -237,18 +237,25 @@ struct Walk {
 // ---------------------------------------------------------------------------
 // Device helpers
 // ---------------------------------------------------------------------------
-// Waits are bounded.  One that runs out sets the CTA's flag and the error word,
+// A wait of any call on this device gave up (captured calls have workspaces that nobody asks).
+__device__ int g_gave_up;
+
+// Waits are bounded.  One that runs out sets the CTA's flag and the error words,
 // and every other wait of the CTA gives up after it.  The lanes of a warp may
 // see that at different polls, so a warp goes on or stops by a vote of its
 // lanes; a warp that stops starts no more copies or products, waits for those
 // it has started (settle) and meets the others at the end of the kernel.
+__device__ __forceinline__ void report(const ChunkParams& p) {
+    atomicExch(p.err, 1);
+    atomicExch(&g_gave_up, 1);
+}
 __device__ __forceinline__ bool ca_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, const ChunkParams& p) {
     for (uint32_t i = 0; i < p.polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 255u && *abort_flag) return false;
     }
     *abort_flag = 1;
-    atomicExch(p.err, 1);
+    report(p);
     return false;
 }
 // the same answer for the whole warp
@@ -259,7 +266,7 @@ __device__ __forceinline__ bool ca_wait_all(uint32_t bar, uint32_t parity, volat
 __device__ __forceinline__ void settle(uint32_t bar, uint32_t parity, const ChunkParams& p) {
     for (uint32_t i = 0; i < kCaPolls; ++i)
         if (mbar_try_wait(bar, parity)) return;
-    atomicExch(p.err, 1);
+    report(p);
 }
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("{\n\t.reg .b64 st;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 st, [%0], %1;\n\t}" ::"r"(bar),
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 
     if (sb & 1023u) {   // the swizzled tiles need 1 KB alignment
         if (tid == 0) {
-            atomicExch(p.err, 1);
+            report(p);
             p.rec[cta * 2] = p.rec[cta * 2 + 1] = make_int4(0, 0, 0, 0);
         }
         return;
@@ -741,7 +748,7 @@ __global__ void __launch_bounds__(kCaThreads, 1)
                     if (!more) s.n = 0;
                     // a segment may take long: look for a free slot now and then
                     for (uint32_t i = 0; run && !mbar_try_wait(seg_empty(seg), seg_phase ^ 1u); ++i) {
-                        if (i + 1 == kSegPolls) *abort_flag = 1, atomicExch(p.err, 1);
+                        if (i + 1 == kSegPolls) *abort_flag = 1, report(p);
                         run = !*abort_flag;
                         __nanosleep(200);
                     }
@@ -1373,6 +1380,19 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t
                           : launch_chunk<FADE_F16, 128>(tq, tk, tv, p, G, s);
     return d->D == 64 ? launch_chunk<FADE_BF16, 64>(tq, tk, tv, p, G, s)
                       : launch_chunk<FADE_BF16, 128>(tq, tk, tv, p, G, s);
+}
+
+extern "C" int fade_chunk_attn_check(void* stream) {
+    void* word = nullptr;
+    FADE_CUDA_TRY(cudaGetSymbolAddress(&word, g_gave_up));
+    int h = 0;
+    cudaStream_t s = as_stream(stream);
+    FADE_CUDA_TRY(cudaMemcpyAsync(&h, word, sizeof(int), cudaMemcpyDeviceToHost, s));
+    FADE_CUDA_TRY(cudaStreamSynchronize(s));
+    if (h == 0) return FADE_OK;
+    FADE_CUDA_TRY(cudaMemsetAsync(word, 0, sizeof(int), s));
+    FADE_CUDA_TRY(cudaStreamSynchronize(s));
+    return FADE_ERR_TIMEOUT;
 }
 
 extern "C" int fade_set_wait_polls(int64_t polls) {

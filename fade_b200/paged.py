@@ -324,8 +324,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     kv_len is never used, and a NaN or infinity in a token's K or V reaches only
     the queries that see the token.  `out` must not overlap q.  Workspace is cached per
     (device, stream, head_dim); calls on one stream, from any number of host
-    threads, follow one another whole, so sharing it is safe.  Graphs captured on one stream share it too: replay them in order, and
-    call once on that stream before the first capture."""
+    threads, follow one another whole, so sharing it is safe.  A captured call's
+    workspace belongs to its graph."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if dev != _lib._current():
         with _lib.on_device(dev):
@@ -372,13 +372,17 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
         *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"), _int32(kv_lens, (R,), "kv_lens"))
     lib = _lib.load()
     st = _lib._stream(dev)
-    ws = _WS.get((dev, st, D))
+    # a graph may be replayed beside anything, so its calls share no workspace with others'
+    captured = _lib._capturing()
+    ws = None if captured else _WS.get((dev, st, D))
     if ws is None:
         need = lib.fade_chunk_attn_workspace_size(d)
         if need == 0:
             raise ValueError(f"unsupported chunk attention sizes (R={R}, T={T}, n_pages={n_pages}, table width {width})")
-        ws = torch.zeros(need, dtype=torch.uint8, device=q.device)
-        ws = _WS.setdefault((dev, st, D), (ws, ws.data_ptr(), need))     # another thread's, if it was first
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        ws = (ws, ws.data_ptr(), need)
+        if not captured:
+            ws = _WS.setdefault((dev, st, D), ws)     # another thread's, if it was first
     code = lib.fade_chunk_attn(d, ws[1], ws[2], st)
     if code:
         _lib.check(code, "chunk_attention")
@@ -386,15 +390,11 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
 
 
 def check_device_errors(device: torch.device | str = "cuda") -> None:
-    """Raise if a bounded device wait of an earlier ``chunk_attention`` call on
-    the current stream gave up (synchronises)."""
-    device = torch.device(device)
-    with _lib.on_device(device) as st:
-        dev = _lib._current()
-        for key, (_, ptr, need) in list(_WS.items()):
-            if key[:2] == (dev, st):
-                status = _lib.load().fade_workspace_check(ptr, need, st)
-                _lib.check(status, "chunk_attention")
+    """Raise if a bounded device wait of a ``chunk_attention`` call on `device`
+    gave up since this was last asked, in a replayed graph or not.  Synchronises
+    the current stream; calls on others are covered once they have ended."""
+    with _lib.on_device(torch.device(device)) as st:
+        _lib.check(_lib.load().fade_chunk_attn_check(st), "chunk_attention")
 
 
 # ---------------------------------------------------------------------------

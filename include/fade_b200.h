@@ -458,15 +458,22 @@ typedef struct fade_chunk_desc {
 } fade_chunk_desc;
 
 /* Bytes of workspace fade_chunk_attn needs for `d` (0: unsupported), 32-byte
- * aligned.  Zero-fill it once when allocating it; fade_workspace_check reads its
- * error word.  Calls may share a workspace on one stream, from several host
- * threads too; calls on different streams may not. */
+ * aligned.  Zero-fill it once when allocating it if fade_workspace_check is to
+ * read its error word (the kernels only write it); fade_chunk_attn_check needs no
+ * workspace.  Calls may share a workspace on one stream, from several host
+ * threads too; calls on different streams, and graphs that may be replayed at the
+ * same time, may not. */
 size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d);
 int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream);
 
+/* Reads and clears the current device's own error word: FADE_ERR_TIMEOUT if a
+ * bounded wait of any fade_chunk_attn call gave up since it was last asked, with
+ * any workspace, captured in a graph or not.  Synchronises `stream`; what runs on
+ * other streams is covered once it has ended. */
+int fade_chunk_attn_check(void* stream);
+
 /* Polls after which a device wait of later fade_chunk_attn calls gives up (the
- * call then ends, its outputs are undefined and the workspace's error word is
- * set): 0 to 2^22, the default; negative: the default again.  Process-wide.  A
+ * call then ends, its outputs are undefined and the error words are set): 0 to 2^22, the default; negative: the default again.  Process-wide.  A
  * low number makes waits run out that would have ended, so that a host's handling
  * of the error can be exercised. */
 int fade_set_wait_polls(int64_t polls);

@@ -27,7 +27,7 @@ class _Devices:
         monkeypatch.setattr(_lib, "_stream", lambda idx: 0)           # the default stream has the same handle on both
         monkeypatch.setattr(torch.cuda, "current_device", lambda: self.now)
         monkeypatch.setattr(torch.cuda, "set_device", self._set)
-        monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+        monkeypatch.setattr(_lib, "_capturing", lambda: False, raising=False)
         monkeypatch.setattr(_lib, "same_device", lambda *t: 1)
         monkeypatch.setattr(_lib, "require_cuda", lambda *t: torch.device("cuda", 1))
 

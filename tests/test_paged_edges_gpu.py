@@ -146,3 +146,94 @@ def test_tiered_decode_attention_from_threads_on_one_stream(cuda_device):
     results = _in_threads([lambda b=b: tiered_decode_attention(*b) for b in batches], 60, torch.cuda.default_stream())
     for want, got in zip(alone, results):
         assert len(got) == 60 and all(torch.equal(g, want) for g in got)
+
+
+def test_captured_calls_report_their_errors(cuda_device):
+    """A wait that gives up in a replayed graph is found from any stream, without the stream of the capture."""
+    from fade_b200 import _lib
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    args = _attn_inputs([3, 1], [900, 40], 8, 2, 64, 16, HF, cuda_device, 34)
+    want = chunk_attention(*args)
+    graph, broken = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    try:
+        assert _lib.load().fade_set_wait_polls(0) == _lib.FADE_OK
+        with torch.cuda.graph(broken):
+            chunk_attention(*args)
+    finally:
+        assert _lib.load().fade_set_wait_polls(-1) == _lib.FADE_OK
+    with torch.cuda.graph(graph):
+        out = chunk_attention(*args)
+    graph.replay()
+    check_device_errors(cuda_device)
+    assert torch.equal(out, want)
+    broken.replay()
+    with pytest.raises(RuntimeError, match="timed out"):
+        check_device_errors(cuda_device)
+    graph.replay()
+    check_device_errors(cuda_device)
+    assert torch.equal(out, want)
+
+
+def test_graphs_replayed_at_the_same_time(cuda_device):
+    """Graphs captured on one stream and replayed on several, beside direct calls: each has its own workspace."""
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    batches = [_attn_inputs(new, kv, 8, 2, 128, 32, BF, cuda_device, 60 + i) for i, (new, kv) in enumerate(
+        (([1, 1, 1], [5000, 900, 2000]), ([200], [2500]), ([40, 1, 70], [1000, 7000, 70])))]
+    alone = [chunk_attention(*b) for b in batches]
+    graphs = []
+    for b in batches:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = chunk_attention(*b)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    for _ in range(40):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        direct = [chunk_attention(*b) for b in batches]
+    torch.cuda.synchronize()
+    check_device_errors(cuda_device)
+    for want, (_, out), also in zip(alone, graphs, direct):
+        assert torch.equal(out, want) and torch.equal(also, want)
+
+
+def test_captured_cache_step(cuda_device):
+    """A whole decode step of PagedKVCache in a graph: replays advance the cache as direct steps do."""
+    from fade_b200.paged import PagedKVCache
+
+    L, hq, hkv, D, R = 2, 8, 2, 64, 3
+    g = torch.Generator(device="cuda").manual_seed(70)
+    inv = (10000.0 ** -(torch.arange(D // 2, device=cuda_device) / (D // 2))).float()
+    prompt = torch.tensor([20, 33, 7], dtype=torch.int32, device=cuda_device)
+    one = torch.ones(R, dtype=torch.int32, device=cuda_device)
+    first = [torch.randn(L, 60, h, D, generator=g, device=cuda_device).to(BF) for h in (hq, hkv, hkv)]
+    steps = [[torch.randn(L, R, h, D, generator=g, device=cuda_device).to(BF) for h in (hq, hkv, hkv)] for _ in range(20)]
+
+    def step(cache, qkv, lens, total):
+        plan = cache.plan(lens, total)
+        return torch.stack([cache.attend(i, plan, cache.append(i, plan, qkv[0][i], qkv[1][i], qkv[2][i], inv))
+                            for i in range(L)])
+
+    caches = [PagedKVCache(L, hkv, D, n_pages=20, max_requests=R, max_tokens=64, page_size=16, dtype=BF,
+                           device=cuda_device) for _ in range(2)]
+    for c in caches:
+        step(c, first, prompt, 60)
+    static = [x.clone() for x in steps[0]]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = step(caches[1], static, one, R)
+    for qkv in steps:
+        want = step(caches[0], qkv, one, R)
+        for s, x in zip(static, qkv):
+            s.copy_(x)
+        graph.replay()
+        assert torch.equal(out, want)
+    for c in caches:
+        c.check()
+        assert c.kv_lens.tolist() == [40, 53, 27]
+    assert torch.equal(caches[0].n_free, caches[1].n_free) and torch.equal(caches[0].k, caches[1].k)
