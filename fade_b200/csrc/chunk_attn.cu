@@ -1295,9 +1295,16 @@ extern "C" size_t fade_chunk_attn_workspace_size(const fade_chunk_desc* d) {
     return ws_bytes_for(G > 0 ? G : 148, d->D);
 }
 
-extern "C" int fade_chunk_attn(const fade_chunk_desc* d, void* workspace, size_t ws_bytes, void* stream) {
-    const int bad = check_desc(d);
+extern "C" int fade_chunk_attn(const fade_chunk_desc* desc, void* workspace, size_t ws_bytes, void* stream) {
+    const int bad = check_desc(desc);
     if (bad != FADE_OK) return bad;
+    // the stride of a dimension of one is never stepped and may be anything: dense ones in their place
+    fade_chunk_desc dense = *desc;
+    const fade_chunk_desc* d = &dense;
+    if (d->Hq == 1) dense.q_sh = dense.o_sh = d->D;
+    if (d->T == 1) dense.q_st = dense.o_st = d->Hq * d->D;
+    if (d->Hkv == 1) dense.kp_sh = dense.vp_sh = d->page_size * d->D;
+    if (d->n_pages <= 1) dense.kp_sp = dense.vp_sp = d->Hkv * d->page_size * d->D;
     if (d->T == 0 || d->R == 0) return FADE_OK;
     if (!d->q || !d->out || !d->cu_q || !d->kv_lens || (d->table_width > 0 && !d->block_table) ||
         (d->n_pages > 0 && (!d->k_pool || !d->v_pool)))

@@ -441,8 +441,8 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * used, whatever they hold; a NaN or infinity in the cache reaches only the
  * queries that see its token.  out must not overlap q.
  * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
- * every pointer and stride of q, k_pool, v_pool and out a multiple of 16 bytes
- * (else FADE_ERR_ALIGN), 0 < sm_scale <= 1e30. */
+ * every pointer and stride (of a dimension of more than one) of q, k_pool, v_pool
+ * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 0 < sm_scale <= 1e30. */
 typedef struct fade_chunk_desc {
     int64_t dtype, R, T, Hq, Hkv, D, page_size, n_pages, table_width, table_stride;
     int64_t causal, window;

@@ -237,3 +237,40 @@ def test_captured_cache_step(cuda_device):
         c.check()
         assert c.kv_lens.tolist() == [40, 53, 27]
     assert torch.equal(caches[0].n_free, caches[1].n_free) and torch.equal(caches[0].k, caches[1].k)
+
+
+def test_strides_that_are_never_stepped(cuda_device):
+    """A dimension of one may have any stride: a token out of a wider row, a pool of one page or one head."""
+    from fade_b200.paged import chunk_attention
+
+    dev = cuda_device
+    q, kp, vp, table, cu, kl = _attn_inputs([1], [40], 2, 1, 64, 64, HF, dev, 35)
+    want = chunk_attention(q, kp, vp, table, cu, kl)
+    rows = torch.zeros(5, 132, dtype=HF, device=dev)
+    rows[2, :128] = q.view(-1)
+    one = rows[:, :128].unflatten(1, (2, 64))[2:3]
+    assert one.stride() == (132, 64, 1)
+    assert torch.equal(chunk_attention(one, kp, vp, table, cu, kl), want)
+    wide = torch.full((3, 2 * 64 + 5), 3.0, dtype=HF, device=dev)
+    dest = wide[:, :128].unflatten(1, (2, 64))[:1]
+    assert dest.stride()[0] % 8 and chunk_attention(q, kp, vp, table, cu, kl, out=dest) is dest
+    assert torch.equal(dest, want) and (wide[1:] == 3).all() and (wide[:, 128:] == 3).all()
+    # a token at an odd address is copied, from its odd stride too
+    flat = torch.zeros(129, dtype=HF, device=dev)
+    flat[1:] = q.view(-1)
+    odd = flat.as_strided((1, 2, 64), (131, 64, 1), 1)
+    assert torch.equal(chunk_attention(odd, kp, vp, table, cu, kl), want)
+    # one head of its own: [T, 1, D] and pools [pages, 1, page, D]
+    page = int(table[0, 0])
+    zero = torch.zeros_like(table)
+    single = [torch.zeros(64 * 64 + 12, dtype=HF, device=dev) for _ in range(2)]
+    for s, p in zip(single, (kp, vp)):
+        s[:64 * 64] = p[page, 0].reshape(-1)
+    k1, v1 = (s.as_strided((1, 1, 64, 64), (4099, 4097, 64, 1)) for s in single)
+    assert torch.equal(chunk_attention(q, k1, v1, zero, cu, kl), want)
+    thin = q[:, :1].clone().as_strided((1, 1, 64), (77, 33, 1))
+    assert torch.equal(chunk_attention(thin, kp, vp, table, cu, kl), chunk_attention(q[:, :1].clone(), kp, vp, table, cu, kl))
+    # broadcast tokens and heads
+    for b in (q[:, :1].expand(1, 2, 64), q.expand(3, 2, 64)):
+        n = torch.tensor([0, b.shape[0]], dtype=torch.int32, device=dev)
+        assert torch.equal(chunk_attention(b, kp, vp, table, n, kl), chunk_attention(b.clone(), kp, vp, table, n, kl))
