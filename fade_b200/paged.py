@@ -429,7 +429,8 @@ class PagedKVCache:
         self._state = torch.zeros(max_requests + 1, dtype=torch.int32, device=dev)
         self._state[-1] = n_pages
         self.kv_lens, self.n_free = self._state[:-1], self._state[-1:]
-        self._release_status = torch.zeros(1, dtype=torch.int32, device=dev)
+        # of the last release, and the worst since `check`
+        self._released, self._release_status = torch.zeros(2, 1, dtype=torch.int32, device=dev)
 
     def plan(self, new_lens: Tensor, total: int, out: StepPlan | None = None) -> StepPlan:
         """Plan a step of ``new_lens`` (int32 [max_requests]) and take its
@@ -457,14 +458,17 @@ class PagedKVCache:
         return chunk_attention(q, self.k[layer], self.v[layer], self.block_table, plan.cu_q, plan.kv_lens, **kw)
 
     def release(self, rows: Tensor) -> None:
-        """Drop the requests of the bool [max_requests] mask `rows`."""
-        release_rows(rows, self.kv_lens, self.block_table, self.page_size, self.free_pages, self.n_free,
-                     self._release_status)
+        """Drop the requests of the bool [max_requests] mask `rows`.  A release
+        that fails drops none of them; ``check`` raises on it, also after others."""
+        release_rows(rows, self.kv_lens, self.block_table, self.page_size, self.free_pages, self.n_free, self._released)
+        torch.maximum(self._release_status, self._released, out=self._release_status)
 
     def check(self) -> None:
-        """Raise if a release failed or a device wait gave up (synchronises)."""
+        """Raise if a release failed or a device wait gave up since the last
+        check (synchronises)."""
         code = int(self._release_status.item())
         if code:
+            self._release_status.zero_()
             raise RuntimeError(f"release: {_PLAN_ERRORS.get(code, f'status {code}')}")
         check_device_errors(self._state.device)
 

@@ -274,3 +274,30 @@ def test_strides_that_are_never_stepped(cuda_device):
     for b in (q[:, :1].expand(1, 2, 64), q.expand(3, 2, 64)):
         n = torch.tensor([0, b.shape[0]], dtype=torch.int32, device=dev)
         assert torch.equal(chunk_attention(b, kp, vp, table, n, kl), chunk_attention(b.clone(), kp, vp, table, n, kl))
+
+
+def test_a_failed_release_is_remembered(cuda_device):
+    """The status of a release outlives the releases after it, until it was looked at."""
+    from fade_b200.paged import PagedKVCache, release_rows
+
+    cache = PagedKVCache(1, 2, 64, n_pages=8, max_requests=2, max_tokens=64, page_size=16, dtype=BF, device=cuda_device)
+    cache.plan(torch.tensor([20, 30], dtype=torch.int32, device=cuda_device), 50).check()
+    first, second = (torch.tensor(m, device=cuda_device) for m in ([True, False], [False, True]))
+    for lens, text in ((65, "row"), (-1, "negative")):          # a page more than a row of the table holds; no length
+        cache.kv_lens[0] = lens
+        cache.release(first)                                     # fails: nothing changes
+        assert cache.kv_lens.tolist() == [lens, 30] and cache.n_free.item() == 4
+        cache.kv_lens[0] = 20
+        cache.release(torch.zeros_like(first))                   # succeeds
+        with pytest.raises(RuntimeError, match=text):
+            cache.check()
+        cache.check()
+    cache.release(first)
+    cache.release(second)
+    cache.check()
+    assert cache.kv_lens.tolist() == [0, 0] and cache.n_free.item() == 8
+    assert sorted(cache.free_pages.tolist()) == list(range(8))
+    # the operator's own status: a negative length of a row that stays counts, too
+    kv = torch.tensor([16, -3], dtype=torch.int32, device=cuda_device)
+    assert release_rows(first, kv, cache.block_table, 16, cache.free_pages, cache.n_free).item() == 4
+    assert kv.tolist() == [16, -3] and cache.n_free.item() == 8
