@@ -45,7 +45,7 @@ class TinyDecoder:
         self.qkv = [weight(width, (n_q_heads + 2 * n_kv_heads) * head_dim) for _ in range(n_layers)]
         self.out = [weight(width, width) for _ in range(n_layers)]
         self.rope = MRope(theta=10000.0, head_dim=head_dim, mrope_section=[8, 12, 12])
-        self.inv_freq = self.rope.inv_freq(torch.device(device))
+        self.inv_freq = self.rope.axes_inv_freq(torch.device(device))
 
     def step(self, cache: PagedKVCache, tokens: Tensor, positions: Tensor, new_lens: Tensor, queries=None) -> Tensor:
         """One step: tokens [T] of the requests one after the other (new_lens

@@ -218,8 +218,9 @@ def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, 
     """Rotary embedding with one to four position axes (time, height, width).
 
     x: [T, H, D] fp16, bf16 or fp32, any token and head strides; positions:
-    integer [A, T] ([T] for one axis); inv_freq: float32 [rot/2] (a
-    ``RopeScheme.inv_freq``); sections: frequencies per axis, see
+    integer [A, T] ([T] for one axis); inv_freq: float32 [rot/2] (a scheme's
+    ``RopeScheme.axes_inv_freq``; its ``inv_freq`` belongs to its tables and
+    differs for scaled positions and models without rotation); sections: frequencies per axis, see
     ``section_axes`` (default: all on one axis).  Channel j pairs with
     ``j + rot/2``; channels from rot on are copied.  ``inverse`` rotates back.
     Angles, cos and sin are fp32 and the result is rounded once;

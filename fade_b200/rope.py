@@ -62,6 +62,12 @@ class RopeScheme:
             self._inv[key] = self._compute_inv_freq(key)
         return self._inv[key]
 
+    def axes_inv_freq(self, device) -> Tensor:
+        """The frequencies for ``fade_b200.paged.rope_axes`` and ``rope_append``,
+        which multiply them by positions as they are: those of ``inv_freq``
+        unless the scheme treats positions otherwise."""
+        return self.inv_freq(device)
+
     def _angles(self, positions: Tensor, device) -> Tensor:
         f = positions.to(device).float()[:, None] * self.inv_freq(device)[None, :]
         return torch.cat((f, f), dim=-1)
@@ -85,6 +91,11 @@ class LinearScaled(RopeScheme):
     """Positions divided by ``factor``."""
 
     factor: float = DEFAULT_FACTOR
+
+    def axes_inv_freq(self, device) -> Tensor:
+        """``inv_freq / factor``: the integer positions of a step cannot carry
+        the division (the angles are off the tables' by fp32 rounding)."""
+        return self.inv_freq(device) / self.factor
 
     def compute_cos_sin(self, positions, device, model_dtype=torch.float16):
         f = (positions.to(device).float() / self.factor)[:, None] * self.inv_freq(device)[None, :]
@@ -167,8 +178,13 @@ class MRope(RopeScheme):
     the tables are vanilla RoPE over ``rotary_dim`` (zero angles beyond).
     Positions of several axes ([A, S], time, height, width) give each
     frequency the angle of its axis: ``mrope_section`` frequencies per axis in
-    order, or ``interleaved`` (``fade_b200.paged.rope_axes`` applies the same
-    angles without tables)."""
+    order, or ``interleaved``.
+
+    ``fade_b200.paged.rope_axes`` applies the same rotation without tables where
+    ``partial_rotary_factor`` is 1.  Below 1 it pairs channel j with ``j +
+    rotary_dim/2``, as models do; these tables are the reference's, (f, f, 0)
+    over the whole head, for a re-RoPE that pairs j with ``j + head_dim/2``.
+    Keys rotated by the one cannot be un-rotated by the other."""
 
     partial_rotary_factor: float = 1.0
     mrope_section: list | None = None
@@ -201,6 +217,10 @@ class MRope(RopeScheme):
 @dataclass
 class NoRope(RopeScheme):
     """Models without rotary embeddings: identity tables."""
+
+    def axes_inv_freq(self, device) -> Tensor:
+        """No frequencies: nothing turns."""
+        return torch.empty(0, dtype=torch.float32, device=device)
 
     def compute_cos_sin(self, positions, device, model_dtype=torch.float16):
         S = positions.shape[0]

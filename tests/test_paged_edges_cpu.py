@@ -89,3 +89,28 @@ def test_calls_run_on_their_tensors_device(monkeypatch, op):
         call()
         assert lib.seen and set(lib.seen) == {1}
         assert lib.now == 0
+
+
+def _schemes():
+    from fade_b200 import rope
+
+    return [rope.Vanilla(head_dim=16), rope.LinearScaled(head_dim=16, factor=4.0), rope.LinearScaled(head_dim=16, factor=3.0),
+            rope.Llama3(head_dim=16, factor=8.0), rope.NtkAware(head_dim=16, factor=2.0), rope.Yarn(head_dim=16, factor=4.0),
+            rope.Proportional(head_dim=16, partial_rotary_factor=0.5), rope.MRope(head_dim=16, mrope_section=[2, 3, 3]),
+            rope.NoRope(head_dim=16)]
+
+
+@pytest.mark.parametrize("scheme", _schemes(), ids=lambda s: type(s).__name__)
+def test_step_frequencies_give_the_schemes_tables(scheme):
+    """cos and sin of position * axes_inv_freq are what the scheme's own tables hold, for every scheme."""
+    pos = torch.tensor([0, 1, 17, 1000, 30011])
+    cos, sin = scheme.compute_cos_sin(pos, "cpu", model_dtype=torch.float32)
+    f = scheme.axes_inv_freq("cpu")
+    assert f.dtype == torch.float32 and f.numel() in (0, 8)
+    angle = torch.zeros(5, 8)
+    angle[:, :f.numel()] = pos.float()[:, None] * f
+    # two roundings of the angle either way, and of cos and sin
+    lim = 4 * 2.0 ** -24 * angle.abs() + 2.0 ** -22
+    for half in (slice(0, 8), slice(8, 16)):
+        assert ((angle.double().cos() - cos[0, 0, :, half]).abs() <= lim).all()
+        assert ((angle.double().sin() - sin[0, 0, :, half]).abs() <= lim).all()

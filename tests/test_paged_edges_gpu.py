@@ -301,3 +301,25 @@ def test_a_failed_release_is_remembered(cuda_device):
     kv = torch.tensor([16, -3], dtype=torch.int32, device=cuda_device)
     assert release_rows(first, kv, cache.block_table, 16, cache.free_pages, cache.n_free).item() == 4
     assert kv.tolist() == [16, -3] and cache.n_free.item() == 8
+
+
+def test_rope_axes_of_every_scheme(cuda_device):
+    """rope_axes with a scheme's step frequencies against its tables, in the tier cache's pairing (j, j + D/2)."""
+    from fade_b200 import rope
+    from fade_b200.paged import rope_axes
+
+    g = torch.Generator(device="cuda").manual_seed(80)
+    D, x = 64, torch.randn(40, 3, 64, generator=g, device=cuda_device)
+    pos = torch.randint(0, 30000, (40,), generator=g, device=cuda_device)
+    for scheme in (rope.Vanilla(head_dim=D), rope.LinearScaled(head_dim=D, factor=3.0), rope.Llama3(head_dim=D, factor=8.0),
+                   rope.NtkAware(head_dim=D, factor=2.0), rope.Yarn(head_dim=D, factor=4.0),
+                   rope.Proportional(head_dim=D, partial_rotary_factor=0.5),
+                   rope.MRope(head_dim=D, mrope_section=[32]), rope.NoRope(head_dim=D)):
+        f = scheme.axes_inv_freq(cuda_device)
+        cos, sin = (t[0, 0].double()[:, None] for t in scheme.compute_cos_sin(pos, cuda_device, model_dtype=torch.float32))
+        a, b = x.double().split(D // 2, -1)
+        want = torch.cat([a * cos[..., :D // 2] - b * sin[..., :D // 2], b * cos[..., D // 2:] + a * sin[..., D // 2:]], -1)
+        angle = torch.zeros(40, 1, D // 2, device=cuda_device)
+        angle[:, 0, :f.numel()] = pos.float()[:, None] * f
+        lim = (a.abs() + b.abs()) * (4 * 2.0 ** -24 * angle + 2.0 ** -21)
+        assert ((rope_axes(x, pos, f).double() - want).abs() <= torch.cat([lim, lim], -1)).all(), type(scheme).__name__
