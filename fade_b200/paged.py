@@ -13,8 +13,9 @@ no host synchronisation:
   tokens to long prompt chunks, causal and optionally windowed.
 
 ``PagedKVCache`` owns the pool, table and free list and strings the three
-together; ``gather`` hands a request's K/V on to the tier quantisers
-(``TieredDecoder.load_prompt``, ``TieredKVCache.update``).
+together; ``gather`` hands a request's K/V on to the tier quantisers:
+``TieredDecoder.load_prompt``, and ``TieredKVCache.update`` for requests at text
+positions (see there).
 
 The reference keeps one dense cache per batch and has no counterpart.
 """
@@ -476,7 +477,13 @@ class PagedKVCache:
     def gather(self, layer: int, rows, length: int) -> tuple[Tensor, Tensor]:
         """K, V [len(rows), n_kv_heads, length, head_dim] of the first `length`
         tokens of the given rows, contiguous: what the tier quantisers and
-        ``TieredDecoder.load_prompt`` take."""
+        ``TieredDecoder.load_prompt`` take.
+
+        K comes as it was rotated.  ``TieredDecoder`` keeps it so, whatever its
+        positions were.  ``TieredKVCache`` un-rotates what an eviction leaves, and
+        has one position per token for it, counted from 0: hand it only requests
+        that were appended at the plan's own positions (no ``positions``), not those
+        with image or video tokens on several axes."""
         pages = self.block_table[rows, :-(-length // self.page_size)].long()
         return tuple(p[layer][pages].transpose(1, 2).flatten(2, 3)[:, :, :length].contiguous()
                      for p in (self.k, self.v))

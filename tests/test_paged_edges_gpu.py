@@ -323,3 +323,40 @@ def test_rope_axes_of_every_scheme(cuda_device):
         angle[:, 0, :f.numel()] = pos.float()[:, None] * f
         lim = (a.abs() + b.abs()) * (4 * 2.0 ** -24 * angle + 2.0 ** -21)
         assert ((rope_axes(x, pos, f).double() - want).abs() <= torch.cat([lim, lim], -1)).all(), type(scheme).__name__
+
+
+def test_hand_over_to_the_tier_cache_at_text_positions(cuda_device):
+    """Pages gathered into TieredKVCache go through an eviction (un-rotated and rotated again) as the model's own keys do."""
+    from fade_b200.cache import TieredKVCache
+    from fade_b200.paged import PagedKVCache
+    from fade_b200.policy import _assign_one_layer
+    from fade_b200.rope import LinearScaled
+
+    g = torch.Generator(device="cuda").manual_seed(90)
+    hq, hkv, D, n = 4, 2, 64, 150
+    scheme = LinearScaled(theta=10000.0, head_dim=D, factor=2.0)
+    q, k, v = (torch.randn(n, h, D, generator=g, device=cuda_device).half() for h in (hq, hkv, hkv))
+    pages = PagedKVCache(1, hkv, D, n_pages=16, max_requests=2, max_tokens=256, page_size=16, dtype=HF, device=cuda_device)
+    plan = pages.plan(torch.tensor([0, n], dtype=torch.int32, device=cuda_device), n)
+    # sin and cos rounded to fp16 as the scheme's tables are; half of an integer position is exact, so the angles agree
+    pages.append(0, plan, q, k, v, scheme.axes_inv_freq(cuda_device), round_tables=True)
+    plan.check()
+    cos, sin = (t[0, 0][:, None] for t in scheme.compute_cos_sin(torch.arange(n, device=cuda_device), cuda_device, torch.float16))
+    turned = torch.cat([-k[..., D // 2:], k[..., :D // 2]], -1).float()
+    direct = (k.float() * cos + turned * sin).half().transpose(0, 1)[None]
+    caches = []
+    for keys, values in ((direct, v.transpose(0, 1)[None]), pages.gather(0, [1], n)):
+        cache = TieredKVCache(n_sink=4, recent_window=16, int4_budget=40, dtype=HF, rope_theta=10000.0, head_dim=D,
+                              rope_scheme=scheme)
+        cache.update(keys.contiguous(), values.contiguous(), 0)
+        scores = torch.rand(n, generator=torch.Generator(device="cuda").manual_seed(91), device=cuda_device)
+        cache.apply_tier_assignment(0, _assign_one_layer(n, scores, 4, 16, 40, 0))
+        caches.append(cache)
+    a, b = (c._materialize(0) for c in caches)
+    assert a[0].shape == b[0].shape and a[0].shape[2] == 60
+    assert torch.equal(a[1], b[1])
+    # K: one fp16 rounding of the rotation apart, then 4-bit codes of the middle: a step of the scale
+    step = float(a[0].abs().max()) / 7 + 4 * 2.0 ** -11 * float(a[0].abs().max())
+    assert float((a[0] - b[0]).abs().max()) <= step
+    sinks = slice(0, 4)
+    assert float((a[0][:, :, sinks] - b[0][:, :, sinks]).abs().max()) <= 8 * 2.0 ** -11 * float(direct.abs().max())
