@@ -1314,7 +1314,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* desc, void* workspace, siz
         if (s % 8) return FADE_ERR_ALIGN;
     if (!aligned16(d->q) || !aligned16(d->out) || !aligned16(d->k_pool) || !aligned16(d->v_pool)) return FADE_ERR_ALIGN;
     if (!workspace || ws_bytes < fade_chunk_attn_workspace_size(d)) return FADE_ERR_WORKSPACE;
-    if (d->out == d->q) return FADE_ERR_INVALID_ARG;
+    if (views_overlap(d->q, d->q_st, d->q_sh, d->out, d->o_st, d->o_sh, d->T, d->Hq, d->D, 2)) return FADE_ERR_INVALID_ARG;
     if (reinterpret_cast<uintptr_t>(workspace) % 32) return FADE_ERR_ALIGN;   // 32-byte loads and stores of the parts
     const int G = fade_sm_count();
     if (G <= 0) return FADE_ERR_CUDA;

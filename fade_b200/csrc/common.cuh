@@ -60,6 +60,29 @@ template <class Encode> inline bool encoded(const Encode& encode) {
 // then follow one another whole, instead of launch by launch.
 std::mutex& workspace_mutex(const void* workspace);
 
+// Do two [T, H, D] views with contiguous channels (strides in elements of
+// `bytes`) share an element?  Views of other strides count as sharing wherever
+// their ranges meet; equal ones may interleave (parts of one fused tensor).
+inline bool views_overlap(const void* a, int64_t a_st, int64_t a_sh, const void* b, int64_t b_st, int64_t b_sh, int64_t T,
+                          int64_t H, int64_t D, int64_t bytes) {
+    if (T <= 0 || H <= 0 || D <= 0) return false;
+    if (T == 1) a_st = b_st = 0;
+    if (H == 1) a_sh = b_sh = 0;
+    const int64_t x = reinterpret_cast<intptr_t>(a), y = reinterpret_cast<intptr_t>(b);
+    if (x + ((T - 1) * a_st + (H - 1) * a_sh + D) * bytes <= y || y + ((T - 1) * b_st + (H - 1) * b_sh + D) * bytes <= x)
+        return false;
+    if (a_st != b_st || a_sh != b_sh || (y - x) % bytes) return true;
+    // is y - x = t st + h sh + c for some |t| < T, |h| < H, |c| < D?
+    for (int64_t h = 1 - H; h < H; ++h) {
+        const int64_t r = (y - x) / bytes - h * a_sh, t0 = a_st ? r / a_st : 0;
+        for (int64_t t = t0 - 1; t <= t0 + 1; ++t) {
+            const int64_t c = r - t * a_st;
+            if (t > -T && t < T && c > -D && c < D) return true;
+        }
+    }
+    return false;
+}
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -459,6 +459,11 @@ extern "C" int fade_rope_axes(const fade_rope_desc* d, void* stream) {
     if (d->T == 0 || (d->Hq == 0 && d->Hkv == 0)) return FADE_OK;
     if ((d->rot > 0 && (!d->positions || !d->inv_freq)) || (d->Hq > 0 && (!d->q || !d->q_out)))
         return FADE_ERR_INVALID_ARG;
+    // in place, or apart: a block reads what another one may have written otherwise
+    const bool in_place = d->q == d->q_out && (d->T == 1 || d->q_st == d->qo_st) && (d->Hq == 1 || d->q_sh == d->qo_sh);
+    if (!in_place && views_overlap(d->q, d->q_st, d->q_sh, d->q_out, d->qo_st, d->qo_sh, d->T, d->Hq, d->D,
+                                   d->dtype == FADE_F32 ? 4 : 2))
+        return FADE_ERR_INVALID_ARG;
     int pl = 0;
     if (d->Hkv > 0) {
         pl = log2_of(d->page_size);

@@ -403,7 +403,8 @@ int fade_release_rows(const uint8_t* rows, int64_t R, int32_t* kv_lens, const in
  *   y[j] = x[j]*c - x[j+rot/2]*s,  y[j+rot/2] = x[j+rot/2]*c + x[j]*s
  * in fp32 (fused multiply-adds), one rounding at the store;
  * inverse = 1 negates s; channels rot..D-1 are copied.
- * q [T,Hq,D] -> q_out (may be q itself).  With Hkv > 0: k is rotated likewise
+ * q [T,Hq,D] -> q_out (may be q itself, with its strides; another overlap is
+ * FADE_ERR_INVALID_ARG).  With Hkv > 0: k is rotated likewise
  * and, with v as it is, written to cache slot slots[t] of k_pool / v_pool
  * (element (page, head, token) at page*sp + head*sh + token*st); slots outside
  * [0, n_pages * page_size) are dropped.  All strides in elements, channels
@@ -439,7 +440,7 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * key gets 0 and -inf.  Rows of q past cu_q[R] are left alone in out and lse.
  * Cache contents past kv_lens (the rest of the last page, other pages) are never
  * used, whatever they hold; a NaN or infinity in the cache reaches only the
- * queries that see its token.  out must not overlap q.
+ * queries that see its token.  out must not overlap q (FADE_ERR_INVALID_ARG).
  * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
  * every pointer and stride (of a dimension of more than one) of q, k_pool, v_pool
  * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 0 < sm_scale <= 1e30. */

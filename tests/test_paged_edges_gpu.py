@@ -360,3 +360,37 @@ def test_hand_over_to_the_tier_cache_at_text_positions(cuda_device):
     assert float((a[0] - b[0]).abs().max()) <= step
     sinks = slice(0, 4)
     assert float((a[0][:, :, sinks] - b[0][:, :, sinks]).abs().max()) <= 8 * 2.0 ** -11 * float(direct.abs().max())
+
+
+def test_overlapping_outputs_are_refused(cuda_device):
+    """An output that shares elements with the input is refused, one that only lies between them is not."""
+    from fade_b200.paged import chunk_attention, rope_axes
+
+    _, kp, vp, table, cu, kl = _attn_inputs([6, 5], [30, 20], 4, 2, 64, 16, BF, cuda_device, 36)
+    g = torch.Generator(device="cuda").manual_seed(37)
+    pos = torch.arange(11, device=cuda_device)
+    inv = torch.rand(32, generator=g, device=cuda_device)
+
+    def attend(x, out=None):
+        return chunk_attention(x, kp, vp, table, cu, kl, out=out)
+
+    def rotate(x, out=None):
+        return rope_axes(x, pos, inv, out=out)
+
+    for call in (attend, rotate):
+        rows = torch.randn(12, 4, 64, generator=g, device=cuda_device).to(BF)
+        heads = torch.randn(11, 9, 64, generator=g, device=cuda_device).to(BF)
+        turned = torch.randn(4, 11, 64, generator=g, device=cuda_device).to(BF)
+        flat = torch.randn(11 * 4 * 64 + 8, generator=g, device=cuda_device).to(BF)
+        for x, out in ((rows[:-1], rows[1:]), (heads[:, :4], heads[:, 3:7]), (heads[:, :8:2], heads[:, 2:9:2]),
+                       (flat[:-8].view(11, 4, 64), flat[8:].view(11, 4, 64)),
+                       (turned.transpose(0, 1), turned.view(11, 4, 64))):
+            with pytest.raises(ValueError):
+                call(x, out)
+        # the other heads of the same tensor, side by side and alternating
+        for x, out in ((heads[:, :4], heads[:, 4:8]), (heads[:, :8:2], heads[:, 1:8:2]), (heads[:, 1:8:2], heads[:, 2:9:2])):
+            want = call(x.clone())
+            assert torch.equal(call(x, out), want)
+    x = torch.randn(11, 4, 64, generator=g, device=cuda_device).to(BF)
+    want = rotate(x)
+    assert rotate(x, x) is x and torch.equal(x, want)              # in place
