@@ -359,6 +359,24 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+// N results as N / 2 pairs.  An average of fp16 values lies within their range,
+// but with its weights rounded it may pass 65504 by 2^-11 and would round to an
+// infinity: a group that has such a value is rounded towards zero instead
+// (which leaves infinities as they are).
+template <int DT, int N>
+__device__ __forceinline__ void pack_results(const float (&f)[N], uint32_t (&y)[N / 2]) {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) y[j] = pack2<DT>(f[2 * j], f[2 * j + 1]);
+    if constexpr (DT == FADE_F16) {
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(f[j]));
+        if (top > 65504.f) {
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
+        }
+    }
+}
 // 32 bytes of a row: one store where every row is 32-byte aligned (a warp stores 32 rows, each its own cache line,
 // and the lines, not the bytes, bound it)
 template <int N>
@@ -985,7 +1003,8 @@ __global__ void __launch_bounds__(kCaThreads, 1)
 #pragma unroll
                         for (int j = 0; j < 16; ++j) zero = fma2(pair(f[2 * j], f[2 * j + 1]), 0, zero);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) y[j] = pack2<DT>(f[2 * j] * inv, f[2 * j + 1] * inv);
+                        for (int j = 0; j < 32; ++j) f[j] *= inv;
+                        pack_results<DT>(f, y);
 #pragma unroll
                         for (int j = 0; j < 16; j += 8) st_row32(orow_p + c + 2 * j, y, j, p.out32);
                     } else if (valid) {   // [channel / 8][row][8]: consecutive rows next to each other
@@ -1087,7 +1106,11 @@ __device__ __forceinline__ void mend_row(const ChunkParams& p, int b, int h, int
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
 #pragma unroll
-    for (int c = 0; c < N; ++c) out[c] = Elem<DT>::from_f(acc[c] * inv);
+    for (int c = 0; c < N; ++c) acc[c] *= inv;
+    uint32_t y[N / 2];
+    pack_results<DT>(acc, y);
+#pragma unroll
+    for (int c = 0; c < N / 2; ++c) reinterpret_cast<uint32_t*>(out)[c] = y[c];
 }
 // The rows q0, q0 + step, ... below end of a tile
 template <int DT, int D>
@@ -1183,13 +1206,15 @@ __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __gri
         const int64_t t = (int64_t)rec.w + q / p.g;
         const int hq = h * p.g + q % p.g;
         uint32_t y[8];
+        float f[16];
         float zero = 0.f;                                  // NaN if an output is not finite
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            y[2 * j] = pack2<DT>(acc[j].x * inv, acc[j].y * inv);
-            y[2 * j + 1] = pack2<DT>(acc[j].z * inv, acc[j].w * inv);
+            f[4 * j] = acc[j].x * inv, f[4 * j + 1] = acc[j].y * inv;
+            f[4 * j + 2] = acc[j].z * inv, f[4 * j + 3] = acc[j].w * inv;
             zero = fmaf(acc[j].x, 0.f, fmaf(acc[j].y, 0.f, fmaf(acc[j].z, 0.f, fmaf(acc[j].w, 0.f, zero))));
         }
+        pack_results<DT>(f, y);
         bad |= !(zero == 0.f);
         st_row32(static_cast<typename Elem<DT>::T*>(p.out) + t * p.o_st + (int64_t)hq * p.o_sh + c4 * 4, y, 0, p.out32);
         if (p.lse && c4 == 0) p.lse[t * p.Hq + hq] = l == 0.f ? -INFINITY : 0.69314718056f * (m + __log2f(l));

@@ -3,6 +3,7 @@ captured steps, strides that are never stepped, values at the types' limits."""
 
 from __future__ import annotations
 
+import math
 import threading
 
 import pytest
@@ -394,3 +395,33 @@ def test_overlapping_outputs_are_refused(cuda_device):
     x = torch.randn(11, 4, 64, generator=g, device=cuda_device).to(BF)
     want = rotate(x)
     assert rotate(x, x) is x and torch.equal(x, want)              # in place
+
+
+@pytest.mark.parametrize("R,new,D", [(40, 1, 64), (20, 40, 128)])      # one half tile (decodes), two half tiles
+def test_averages_of_the_largest_fp16_values_stay_finite(cuda_device, R, new, D):
+    """Weights are rounded to fp16 for their product with V, their sum is not: 65504 averaged must not become an infinity."""
+    from fade_b200.paged import chunk_attention
+
+    n = 1400
+    q, kp, vp, table, cu, kl = _attn_inputs([new] * R, [n] * R, 32, 8, D, 16, HF, cuda_device, 38, poison=False)
+    # 256 keys of score 0, then equal keys whose weight 1 + 1.01 * 2^-11 against them rounds up to 1 + 2^-10
+    q.zero_(), kp.zero_()
+    q[..., 0] = 1.0
+    j = torch.arange(256, n, device=cuda_device)
+    for r in range(R):
+        kp[table[r].long()[j // 16], :, j % 16, 0] = 1.0
+    vp[..., ::2], vp[..., 1::2] = 65504.0, -65504.0
+    sm = math.log(1 + 1.01 * 2.0 ** -11)
+    want = torch.full((D,), 65504.0, device=cuda_device)
+    want[1::2] = -65504.0
+    out = chunk_attention(q, kp, vp, table, cu, kl, sm_scale=sm)
+    assert out.isfinite().all()
+    # weights rounded: 2^-11 of the value, and the result's own rounding
+    assert ((out.float() - want).abs() <= 65504 * 2.0 ** -10).all()
+    # a visible infinity is one, also beside hidden ones of the other sign that make other rows look again
+    last = table[:, (n - 1) // 16].long()
+    vp[last, :, (n - 1) % 16, 2] = float("inf")
+    out = chunk_attention(q, kp, vp, table, cu, kl, sm_scale=sm).unflatten(0, (R, new))
+    assert (out[:, -1, :, 2] == float("inf")).all()
+    assert out[:, :-1].isfinite().all() and ((out[:, :-1].float() - want).abs() <= 65504 * 2.0 ** -10).all()
+    assert ((out[:, -1].float() - want).abs()[..., 3:] <= 65504 * 2.0 ** -10).all()
