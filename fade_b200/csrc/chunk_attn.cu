@@ -1242,7 +1242,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 ca_encode_fn() {
 
 static int check_desc(const fade_chunk_desc* d) {
     if (!d || d->R < 0 || d->T < 0 || d->Hq < 1 || d->Hkv < 1 || d->Hq % d->Hkv || d->table_width < 0 ||
-        d->n_pages < 0 || d->window < 0 || !(d->sm_scale > 0.0) ||
+        d->n_pages < 0 || d->window < 0 || !(d->sm_scale >= 1e-45) ||   // times log2(e) an fp32 number that is not 0
         !(d->sm_scale <= 1e30))
         return FADE_ERR_INVALID_ARG;
     if (d->dtype != FADE_F16 && d->dtype != FADE_BF16) return FADE_ERR_UNSUPPORTED;

@@ -357,8 +357,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     if window is not None and window < 1:
         raise ValueError(f"window must be at least 1, got {window}")
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
-    if not 0.0 < scale <= 1e30:
-        raise ValueError(f"sm_scale must be positive and at most 1e30, got {sm_scale}")
+    if not 1e-45 <= scale <= 1e30:
+        raise ValueError(f"sm_scale must be 1e-45 (the least that fp32 tells from 0) to 1e30, got {sm_scale}")
     q_st, q_sh, one = q.stride()
     q_ptr = q.data_ptr()
     if one != 1 or q_st % 8 or q_sh % 8 or q_ptr % 16:   # rows must be 16-byte aligned for the kernel's loads

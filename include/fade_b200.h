@@ -443,7 +443,7 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * queries that see its token.  out must not overlap q (FADE_ERR_INVALID_ARG).
  * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
  * every pointer and stride (of a dimension of more than one) of q, k_pool, v_pool
- * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 0 < sm_scale <= 1e30. */
+ * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 1e-45 <= sm_scale <= 1e30 (an fp32 number that is not 0). */
 typedef struct fade_chunk_desc {
     int64_t dtype, R, T, Hq, Hkv, D, page_size, n_pages, table_width, table_stride;
     int64_t causal, window;

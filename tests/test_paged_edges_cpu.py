@@ -114,3 +114,13 @@ def test_step_frequencies_give_the_schemes_tables(scheme):
     for half in (slice(0, 8), slice(8, 16)):
         assert ((angle.double().cos() - cos[0, 0, :, half]).abs() <= lim).all()
         assert ((angle.double().sin() - sin[0, 0, :, half]).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("sm_scale,ok", [(1e-46, False), (5e-324, False), (1e-45, True), (1e-40, True), (1e30, True), (1.1e30, False)])
+def test_scales_that_fp32_cannot_hold_are_refused(sm_scale, ok):
+    """A scale that is 0 in fp32 would make 0 x infinity of every hidden key's score."""
+    import ctypes
+
+    d = _lib.ChunkDesc(dtype=_lib.FADE_BF16, R=1, T=1, Hq=1, Hkv=1, D=64, page_size=16, n_pages=1, table_width=1,
+                       table_stride=1, causal=1, sm_scale=sm_scale)
+    assert (_lib.load().fade_chunk_attn_workspace_size(ctypes.byref(d)) > 0) == ok

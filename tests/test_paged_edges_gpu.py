@@ -425,3 +425,16 @@ def test_averages_of_the_largest_fp16_values_stay_finite(cuda_device, R, new, D)
     assert (out[:, -1, :, 2] == float("inf")).all()
     assert out[:, :-1].isfinite().all() and ((out[:, :-1].float() - want).abs() <= 65504 * 2.0 ** -10).all()
     assert ((out[:, -1].float() - want).abs()[..., 3:] <= 65504 * 2.0 ** -10).all()
+
+
+def test_smallest_scale(cuda_device):
+    """Scores far below any difference: the plain average of the visible values, and no NaN from hidden ones."""
+    from fade_b200.paged import chunk_attention
+
+    q, kp, vp, table, cu, kl = _attn_inputs([30], [200], 4, 2, 64, 16, HF, cuda_device, 39)
+    for sm in (1e-45, 1e-40, 1e-30):
+        out = chunk_attention(q, kp, vp, table, cu, kl, sm_scale=sm)
+        ref, _, lim, _ = _attn_ref(q, kp, vp, table, [30], [200], True, None, sm)
+        assert ((out.double() - ref).abs() <= lim).all()
+    with pytest.raises(ValueError, match="sm_scale"):
+        chunk_attention(q, kp, vp, table, cu, kl, sm_scale=1e-46)
