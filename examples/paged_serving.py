@@ -60,8 +60,7 @@ class TinyDecoder:
             q = cache.append(i, plan, q, k, v, self.inv_freq, self.rope.mrope_section, positions)
             if queries is not None:
                 queries.append(q)
-            # padding tokens are not attended for: they keep zeros
-            o = cache.attend(i, plan, q, out=torch.zeros_like(q))
+            o = cache.attend(i, plan, q)                 # zeros for padding tokens
             hidden = hidden + o.reshape(T, -1) @ self.out[i]
         return hidden
 

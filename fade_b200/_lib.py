@@ -151,7 +151,7 @@ PACK_ROPE = struct.Struct("@7q4q5q2P" + "P2q" * 4 + "P2q" + "P3q" * 2)
 class ChunkDesc(ctypes.Structure):
     _fields_ = [
         *((n, _c_i64) for n in ("dtype", "R", "T", "Hq", "Hkv", "D", "page_size", "n_pages", "table_width",
-                                "table_stride", "causal", "window")),
+                                "table_stride", "causal", "window", "fill_rest")),
         ("sm_scale", ctypes.c_double),
         ("q", _vp), ("q_st", _c_i64), ("q_sh", _c_i64),
         ("out", _vp), ("o_st", _c_i64), ("o_sh", _c_i64),
@@ -162,7 +162,7 @@ class ChunkDesc(ctypes.Structure):
     ]
 
 
-PACK_CHUNK = struct.Struct("@12qd" + "P2q" * 2 + "P" + "P3q" * 2 + "3P")
+PACK_CHUNK = struct.Struct("@13qd" + "P2q" * 2 + "P" + "P3q" * 2 + "3P")
 
 # (name, restype, argtypes) for every symbol of include/fade_b200.h
 _SIGNATURES = {

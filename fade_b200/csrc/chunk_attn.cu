@@ -100,7 +100,7 @@ struct ChunkParams {
     int64_t table_stride, o_st, o_sh, q_st, q_sh, kp_sp, kp_sh, kp_st, vp_sp, vp_sh, vp_st;
     uint32_t tile_magic;   // division by the tokens of a tile
     int tile_shift;
-    int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32;
+    int R, T, Hq, Hkv, g, tq, page_log2, n_pages, table_width, causal, window, out32, fill_rest;
     float scale_log2, lazy;   // lazy: how far a score may exceed the running maximum
     uint32_t polls;           // of a wait before it gives up
 };
@@ -1163,6 +1163,18 @@ constexpr int kJoinThreads = 256;
 template <int DT, int D>
 __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int kRows = kJoinThreads / (D / 16);
+    if (p.fill_rest && blockIdx.x == gridDim.x - 1) {   // rows past the last request, which no tile has
+        for (int t = min(max(p.cu_q[p.R], 0), p.T) + blockIdx.y; t < p.T; t += gridDim.y) {
+            auto* row = static_cast<typename Elem<DT>::T*>(p.out) + (int64_t)t * p.o_st;
+            if (p.fill_rest & 1)
+                for (int i = threadIdx.x; i < p.Hq * (D / 8); i += kJoinThreads)
+                    *reinterpret_cast<uint4*>(row + (int64_t)(i / (D / 8)) * p.o_sh + i % (D / 8) * 8) =
+                        make_uint4(0u, 0u, 0u, 0u);
+            if ((p.fill_rest & 2) && p.lse)
+                for (int i = threadIdx.x; i < p.Hq; i += kJoinThreads) p.lse[(int64_t)t * p.Hq + i] = -INFINITY;
+        }
+        return;
+    }
     griddep_wait();
     const int c = blockIdx.x;
     const int4 rec = p.rec[c * 2], more = p.rec[c * 2 + 1];
@@ -1298,7 +1310,7 @@ static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
     // enough blocks for the rows that a tile can have, few enough to wait beside the first kernel's
     const int64_t rows = std::min<int64_t>(256, (int64_t)p.T * p.g);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(G, (unsigned)std::min<int64_t>(8, (rows * (D / 16) + kJoinThreads - 1) / kJoinThreads));
+    cfg.gridDim = dim3(G + (p.fill_rest ? 1 : 0), (unsigned)std::min<int64_t>(8, (rows * (D / 16) + kJoinThreads - 1) / kJoinThreads));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -1385,6 +1397,7 @@ extern "C" int fade_chunk_attn(const fade_chunk_desc* desc, void* workspace, siz
     p.n_pages = (int)d->n_pages;
     p.table_width = d->n_pages > 0 ? (int)d->table_width : 0;
     p.causal = d->causal != 0;
+    p.fill_rest = (int)(d->fill_rest & 3);
     p.window = d->window >= (1LL << 29) ? 0 : (int)d->window;   // as long as the longest cache: hides nothing
     p.out32 = reinterpret_cast<uintptr_t>(d->out) % 32 == 0 && d->o_st % 16 == 0 && d->o_sh % 16 == 0;
     p.scale_log2 = (float)(d->sm_scale * 1.4426950408889634);

@@ -319,15 +319,18 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
     ``window`` or more before it.  Query head h reads kv head
     ``h // (Hq // Hkv)``; sm_scale defaults to 1/sqrt(D).
 
-    Returns [T, Hq, D] (zeros where no key is visible; tokens past cu_q[R] are
-    not written); with ``return_lse`` a dict of that as "out" and the float32
-    [T, Hq] log of the sum of exponentials as "lse" (-inf where no key is
-    visible).  Head_dim 64 or 128, page size 16 to 128, Hq / Hkv up to 128.  What the pool holds past a request's
-    kv_len is never used, and a NaN or infinity in a token's K or V reaches only
-    the queries that see the token.  `out` must not overlap q.  Workspace is cached per
-    (device, stream, head_dim); calls on one stream, from any number of host
-    threads, follow one another whole, so sharing it is safe.  A captured call's
-    workspace belongs to its graph."""
+    Returns [T, Hq, D], zeros where no key is visible and for tokens past cu_q[R]
+    (which a given `out` keeps); with ``return_lse`` a dict of that as "out" and
+    the float32 [T, Hq] log of the sum of exponentials as "lse", -inf for those
+    rows.  Head_dim 64 or 128, page size 16 to 128, Hq / Hkv up to 128.  What the
+    pool holds past a request's kv_len is never used, and a NaN or infinity in a
+    token's K or V reaches only the queries that see the token (a channel in which
+    a query sees an infinity itself may be NaN).  `out` must not overlap q.
+
+    Workspace is cached per (device, stream, head_dim), 39 MB at head_dim 128;
+    calls on one stream, from any number of host threads, follow one another
+    whole, so sharing it is safe.  A captured call's workspace belongs to its
+    graph."""
     dev = _lib.same_device(q, k_pool, v_pool, block_table, cu_q, kv_lens, q if out is None else out)
     if dev != _lib._current():
         with _lib.on_device(dev):
@@ -366,11 +369,17 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
         if q.data_ptr() % 16:
             q = q.clone()
         (q_st, q_sh, _), q_ptr = q.stride(), q.data_ptr()
+    fresh = out is None
     out, o_st, o_sh = _out_heads(out, q, T, Hq, D)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    if R == 0:                                           # nothing is launched
+        if fresh:
+            out.zero_()
+        if return_lse:
+            lse.fill_(float("-inf"))
     d = _lib.PACK_CHUNK.pack(
         _lib.FADE_BF16 if dtype is torch.bfloat16 else _lib.FADE_F16, R, T, Hq, Hkv, D, page_size, n_pages, width, stride,
-        causal, window or 0, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh, 0 if lse is None else lse.data_ptr(),
+        causal, window or 0, fresh | return_lse << 1, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh, 0 if lse is None else lse.data_ptr(),
         *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"), _int32(kv_lens, (R,), "kv_lens"))
     lib = _lib.load()
     st = _lib._stream(dev)

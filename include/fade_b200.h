@@ -437,7 +437,8 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  *   j < kv_len, causal: j <= p, window > 0: j > p - window.
  * out[t,hq] = softmax(sm_scale q k^T) v over them with kv head hq / (Hq/Hkv),
  * lse (nullable, fp32 [T,Hq]) = log sum exp(sm_scale q k); a query that sees no
- * key gets 0 and -inf.  Rows of q past cu_q[R] are left alone in out and lse.
+ * key gets 0 and -inf.  Rows of q past cu_q[R] are left alone in out and lse,
+ * unless fill_rest says otherwise: bit 0, out gets 0 there; bit 1, lse -inf.
  * Cache contents past kv_lens (the rest of the last page, other pages) are never
  * used, whatever they hold; a NaN or infinity in the cache reaches only the
  * queries that see its token.  out must not overlap q (FADE_ERR_INVALID_ARG).
@@ -446,7 +447,7 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 1e-45 <= sm_scale <= 1e30 (an fp32 number that is not 0). */
 typedef struct fade_chunk_desc {
     int64_t dtype, R, T, Hq, Hkv, D, page_size, n_pages, table_width, table_stride;
-    int64_t causal, window;
+    int64_t causal, window, fill_rest;
     double sm_scale;
     const void* q;      int64_t q_st, q_sh;
     void* out;          int64_t o_st, o_sh;

@@ -438,3 +438,34 @@ def test_smallest_scale(cuda_device):
         assert ((out.double() - ref).abs() <= lim).all()
     with pytest.raises(ValueError, match="sm_scale"):
         chunk_attention(q, kp, vp, table, cu, kl, sm_scale=1e-46)
+
+
+@pytest.mark.parametrize("new,kv,T,hq,hkv,D,dt", [
+    ([3, 0, 2], [40, 9, 700], 5, 8, 2, 64, HF),          # no padding
+    ([3, 0, 2], [40, 9, 700], 37, 8, 2, 128, BF),
+    ([300], [2000], 1024, 14, 2, 64, HF),
+    ([0, 0], [5, 6], 9, 4, 4, 128, BF),                  # a step without tokens (or one that could not be planned)
+])
+def test_tokens_past_the_last_request_are_zeros(cuda_device, new, kv, T, hq, hkv, D, dt):
+    """Fresh outputs hold 0 and -inf for padding tokens, whatever their memory held; a given one keeps its rows."""
+    from fade_b200.paged import check_device_errors, chunk_attention
+
+    q, kp, vp, table, cu, kl = _attn_inputs(new, kv, hq, hkv, D, 16, dt, cuda_device, 41)
+    n = sum(new)
+    ref, ref_lse, lim, lim_lse = _attn_ref(q, kp, vp, table, new, kv, True, None, D ** -0.5)
+    padded = torch.full((T, hq, D), math.nan, dtype=dt, device=cuda_device)
+    padded[:n] = q
+    junk = [torch.full((T, hq, D), math.nan, dtype=dt, device=cuda_device),
+            torch.full((T, hq), math.nan, device=cuda_device)]
+    del junk                                             # the next outputs take this memory
+    out, lse = chunk_attention(padded, kp, vp, table, cu, kl, return_lse=True).values()
+    check_device_errors(cuda_device)
+    assert ((out[:n].double() - ref).abs() <= lim).all() and ((lse[:n].double() - ref_lse).abs() <= lim_lse).all()
+    assert (out[n:] == 0).all() and (lse[n:] == -math.inf).all()
+    mine = torch.full((T, hq + 1, D), 3.0, dtype=dt, device=cuda_device)
+    lse = chunk_attention(padded, kp, vp, table, cu, kl, out=mine[:, 1:], return_lse=True)["lse"]
+    assert torch.equal(mine[:n, 1:], out[:n]) and (mine[n:] == 3).all() and (mine[:, 0] == 3).all()
+    assert (lse[n:] == -math.inf).all()
+    none = torch.zeros(0, table.shape[1], dtype=torch.int32, device=cuda_device)
+    out, lse = chunk_attention(padded, kp, vp, none, cu[:1], kl[:0], return_lse=True).values()
+    assert (out == 0).all() and (lse == -math.inf).all()
