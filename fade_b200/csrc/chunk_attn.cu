@@ -361,8 +361,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 // N results as N / 2 pairs.  An average of fp16 values lies within their range,
 // but with its weights rounded it may pass 65504 by 2^-11 and would round to an
-// infinity: a group that has such a value is rounded towards zero instead
-// (which leaves infinities as they are).
+// infinity: finite results stay within the range.
 template <int DT, int N>
 __device__ __forceinline__ void pack_results(const float (&f)[N], uint32_t (&y)[N / 2]) {
 #pragma unroll
@@ -371,9 +370,10 @@ __device__ __forceinline__ void pack_results(const float (&f)[N], uint32_t (&y)[
         float top = 0.f;
 #pragma unroll
         for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(f[j]));
-        if (top > 65504.f) {
+        if (top > 65504.f) {   // rare
+            auto within = [](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x; };
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y[j]) : "f"(f[2 * j + 1]), "f"(f[2 * j]));
+            for (int j = 0; j < N / 2; ++j) y[j] = pack2<DT>(within(f[2 * j]), within(f[2 * j + 1]));
         }
     }
 }

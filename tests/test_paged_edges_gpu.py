@@ -469,3 +469,17 @@ def test_tokens_past_the_last_request_are_zeros(cuda_device, new, kv, T, hq, hkv
     none = torch.zeros(0, table.shape[1], dtype=torch.int32, device=cuda_device)
     out, lse = chunk_attention(padded, kp, vp, none, cu[:1], kl[:0], return_lse=True).values()
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("new,kv,D", [([300], [900], 128), ([1, 5], [3000, 700], 64)])
+def test_channels_beside_an_infinity_are_what_they_were(cuda_device, new, kv, D):
+    """A visible infinity in one channel changes no bit of the others."""
+    from fade_b200.paged import chunk_attention
+
+    for dt in (HF, BF):
+        q, kp, vp, table, cu, kl = _attn_inputs(new, kv, 8, 2, D, 16, dt, cuda_device, 42)
+        want = chunk_attention(q, kp, vp, table, cu, kl)
+        vp[table[:, 0].long(), :, 0, 5] = float("inf")                # the first token of each request: every row sees it
+        out = chunk_attention(q, kp, vp, table, cu, kl)
+        others = torch.arange(D, device=cuda_device) != 5
+        assert torch.equal(out[..., others], want[..., others]) and not out[..., 5].isfinite().any()
