@@ -32,16 +32,17 @@
 // 11 MMA, 10 walks the tiles and posts the segments.
 //
 // What bounds it, bf16, 32 query and 8 kv heads of 128 channels:
-//   - 4 chunks of 2048 tokens over 8192: 844-875 us, 1.18-1.22 PFLOP/s; tensor
-//     pipe 64 % and exponential unit 64 % of the cycles, at a clock that power
-//     pulls from 1.93 to below 1.75 GHz.  A block of two half tiles takes about
+//   - 4 chunks of 2048 tokens over 8192: 849-888 us, 1.16-1.21 PFLOP/s; tensor
+//     pipe 63 % and exponential unit 63 % of the cycles, at a clock that power
+//     pulls from 1.93 to 1.57 GHz.  A block of two half tiles takes about
 //     3300 cycles against 2048 of its MMAs and 2048 of its exponentials: the
 //     streams' turns at the exponential unit (1400 each) and the chain scores
 //     - maximum - weights - weights x V are of one length.  Without turns
-//     1026 us; half of the exponentials on the FMA pipe instead (twelve
-//     instructions a pair) 995 us against 930 without.
-//   - 16 decodes of up to 8192 tokens: 74.5 us, 5.3 TB/s: HBM while it streams
-//     (5 TMA stages of 32 KB), the rest is start (5 us) and join (4 us).
+//     1026 us against 838; a quarter or half of the exponentials on the FMA pipe
+//     instead (twelve instructions a pair) 930-1094 and 995-1199 us against
+//     912-936.
+//   - 16 decodes of up to 8192 tokens: 73.5 us, 5.4 TB/s: HBM while it streams
+//     (5 TMA stages of 32 KB), the rest is start (5 us), join (4 us), uneven ends.
 //   - 4 chunks of 1021 tokens, window 1024 (fp16): 100 us, 0.69 PFLOP/s: ten
 //     blocks a tile, 2.5 us of output a tile, 10 us of joining.
 //
@@ -1163,7 +1164,9 @@ constexpr int kJoinThreads = 256;
 template <int DT, int D>
 __global__ void __launch_bounds__(kJoinThreads, 3) chunk_join_kernel(const __grid_constant__ ChunkParams p) {
     constexpr int kRows = kJoinThreads / (D / 16);
-    if (p.fill_rest && blockIdx.x == gridDim.x - 1) {   // rows past the last request, which no tile has
+    // Rows past the last request, which no tile has: by blocks of their own, which wait for nothing (as a part of
+    // every block 16 decodes took 1.5 us longer).
+    if (p.fill_rest && blockIdx.x == gridDim.x - 1) {
         for (int t = min(max(p.cu_q[p.R], 0), p.T) + blockIdx.y; t < p.T; t += gridDim.y) {
             auto* row = static_cast<typename Elem<DT>::T*>(p.out) + (int64_t)t * p.o_st;
             if (p.fill_rest & 1)
@@ -1307,10 +1310,12 @@ static int launch_chunk(const CUtensorMap& tq, const CUtensorMap& tk, const CUte
     }
     k<<<G, kCaThreads, CaLayout<D>::BYTES, st>>>(tq, tk, tv, p);
     FADE_LAUNCH_CHECK();
-    // enough blocks for the rows that a tile can have, few enough to wait beside the first kernel's
+    // Blocks for the rows that a tile can have, eight slices at most: they start as the first kernel's CTAs, which
+    // leave no registers beside them, end, and more would queue.  One column more for the rows past the last request.
     const int64_t rows = std::min<int64_t>(256, (int64_t)p.T * p.g);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(G + (p.fill_rest ? 1 : 0), (unsigned)std::min<int64_t>(8, (rows * (D / 16) + kJoinThreads - 1) / kJoinThreads));
+    cfg.gridDim = dim3(G + (p.fill_rest ? 1 : 0),
+                       (unsigned)std::min<int64_t>(8, (rows * (D / 16) + kJoinThreads - 1) / kJoinThreads));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];

@@ -262,7 +262,7 @@ __device__ __forceinline__ int table_at(int j, int turns) {
 // A block makes the cos and sin of `tokens` tokens, then its threads share out
 // their units; the blocks of an SM hide one another's first phase.
 // HBM bound: a token's rows are read and written once.  16384 tokens of 32 + 2
-// x 8 heads of 128 bf16 channels, appended: 73 us, 5.5 TB/s of 403 MB.  With
+// x 8 heads of 128 bf16 channels, appended: 74 us, 5.5 TB/s of 403 MB.  With
 // one head a unit 83 us (more address arithmetic), with four 76 us; three
 // blocks per SM 78 us, five 79 us (spills); with loads under the making of the
 // next tokens' tables 87 us and more (its registers cost blocks).

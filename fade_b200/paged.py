@@ -17,6 +17,8 @@ together; ``gather`` hands a request's K/V on to the tier quantisers:
 ``TieredDecoder.load_prompt``, and ``TieredKVCache.update`` for requests at text
 positions (see there).
 
+Serving only: results carry no gradient, whatever the inputs ask for.
+
 The reference keeps one dense cache per batch and has no counterpart.
 """
 

@@ -441,7 +441,8 @@ int fade_rope_axes(const fade_rope_desc* d, void* stream);
  * unless fill_rest says otherwise: bit 0, out gets 0 there; bit 1, lse -inf.
  * Cache contents past kv_lens (the rest of the last page, other pages) are never
  * used, whatever they hold; a NaN or infinity in the cache reaches only the
- * queries that see its token.  out must not overlap q (FADE_ERR_INVALID_ARG).
+ * queries that see its token (a channel in which a query sees an infinity itself
+ * may be NaN).  out must not overlap q (FADE_ERR_INVALID_ARG).
  * dtype F16 or BF16; D 64 or 128; page_size 16, 32, 64 or 128; Hq/Hkv <= 128;
  * every pointer and stride (of a dimension of more than one) of q, k_pool, v_pool
  * and out a multiple of 16 bytes (else FADE_ERR_ALIGN), 1e-45 <= sm_scale <= 1e30 (an fp32 number that is not 0). */
