@@ -28,7 +28,7 @@ extern "C" const char* fade_status_string(int status) {
     }
 }
 
-extern "C" int fade_version(void) { return 100; }
+extern "C" int fade_version(void) { return 101; }
 
 extern "C" int fade_last_cuda_error(void) { return fade::g_last_cuda_error.load(); }
 

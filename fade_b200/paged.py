@@ -223,8 +223,8 @@ def rope_axes(x: Tensor, positions: Tensor, inv_freq: Tensor, sections=None, *, 
     x: [T, H, D] fp16, bf16 or fp32, any token and head strides; positions:
     integer [A, T] ([T] for one axis); inv_freq: float32 [rot/2] (a scheme's
     ``RopeScheme.axes_inv_freq``; its ``inv_freq`` belongs to its tables and
-    differs for scaled positions and models without rotation); sections: frequencies per axis, see
-    ``section_axes`` (default: all on one axis).  Channel j pairs with
+    differs for scaled positions and models without rotation); sections:
+    frequencies per axis, see ``section_axes`` (default: all on one axis).  Channel j pairs with
     ``j + rot/2``; channels from rot on are copied.  ``inverse`` rotates back.
     Angles, cos and sin are fp32 and the result is rounded once;
     ``round_tables`` rounds cos and sin through x's dtype first, as the tables
@@ -381,7 +381,8 @@ def chunk_attention(q: Tensor, k_pool: Tensor, v_pool: Tensor, block_table: Tens
             lse.fill_(float("-inf"))
     d = _lib.PACK_CHUNK.pack(
         _lib.FADE_BF16 if dtype is torch.bfloat16 else _lib.FADE_F16, R, T, Hq, Hkv, D, page_size, n_pages, width, stride,
-        causal, window or 0, fresh | return_lse << 1, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh, 0 if lse is None else lse.data_ptr(),
+        causal, window or 0, fresh | bool(return_lse) << 1, scale, q_ptr, q_st, q_sh, out.data_ptr(), o_st, o_sh,
+        0 if lse is None else lse.data_ptr(),
         *kp, *vp, bt, _int32(cu_q, (R + 1,), "cu_q"), _int32(kv_lens, (R,), "kv_lens"))
     lib = _lib.load()
     st = _lib._stream(dev)

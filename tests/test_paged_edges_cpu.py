@@ -124,3 +124,15 @@ def test_scales_that_fp32_cannot_hold_are_refused(sm_scale, ok):
     d = _lib.ChunkDesc(dtype=_lib.FADE_BF16, R=1, T=1, Hq=1, Hkv=1, D=64, page_size=16, n_pages=1, table_width=1,
                        table_stride=1, causal=1, sm_scale=sm_scale)
     assert (_lib.load().fade_chunk_attn_workspace_size(ctypes.byref(d)) > 0) == ok
+
+
+def test_return_lse_is_a_truth_value(monkeypatch):
+    from fade_b200 import paged
+
+    _Devices(monkeypatch)
+    monkeypatch.setattr(paged, "_WS", {})
+    i = torch.zeros(1, dtype=torch.int32)
+    x, pool = torch.zeros(1, 1, 64, dtype=torch.float16), torch.zeros(1, 1, 16, 64, dtype=torch.float16)
+    for flag in (None, 0, 1, False, True):
+        got = paged.chunk_attention(x, pool, pool, i[None], torch.zeros(2, dtype=torch.int32), i, return_lse=flag)
+        assert isinstance(got, dict) == bool(flag)
