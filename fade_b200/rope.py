@@ -10,7 +10,7 @@ construction is a few small torch ops on the cache's device.
 Schemes (same names and parameters as the reference): ``Vanilla``,
 ``LinearScaled``, ``Llama3`` (``llama3`` / ``longrope`` scaling), ``NtkAware``
 (``ntk`` / ``dynamic``), ``Yarn``, ``Proportional`` (partial rotation),
-``MRope`` (text-only: shared axes), ``NoRope`` (identity tables).
+``MRope`` (text positions, or one per axis), ``NoRope`` (identity tables).
 """
 
 from __future__ import annotations
